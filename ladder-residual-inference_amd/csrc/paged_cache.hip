@@ -1,0 +1,239 @@
+// lr_paged_write and lr_paged_read: rows of a call into the pages of a key-value cache, and back.
+//
+// Both move every byte once and compute next to nothing: memory-bound, and in a decode step bound by the launch and two dependent
+// reads (where the row belongs, then its page).  A lane has 8 elements of a head's row (16 bytes of bf16), HD / 8 lanes a row.
+#include "paged_common.h"
+
+constexpr int PAGED_TOKENS = 4;   // of a workgroup, at most
+
+// Where a workgroup's tokens belong: sequence, position, page; one wave per token.  page -1: the token is left alone.
+struct PagedPlace {
+  int pos[PAGED_TOKENS], page[PAGED_TOKENS];
+};
+// `limit`: positions from there on have no angle.  A token behind the last sequence, or an empty place of a batch, has no place and is no
+// error; a position or a page that is out of range is one.
+__device__ __forceinline__ void paged_places(const PagedCache& c, const PagedBatch& t, int row0, int rows, int tokens, int limit, PagedPlace& at) {
+  const int wave = threadIdx.x >> 6;
+  if (wave < tokens) {
+    const int row = row0 + wave;
+    int page = -1, pos = 0;
+    if (row < rows) {
+      int b = row, end = row + 1;
+      if (t.starts) {
+        b = paged_sequence(t, row);
+        end = b < t.B ? t.starts[b + 1] : 0;
+      }
+      if (b < t.B) {
+        const int length = t.lengths[b];
+        pos = length - (end - row);
+        int code = 0;
+        if (pos < 0 || pos >> c.shift >= t.pages || pos >= limit) {
+          code = t.starts || length != 0 ? LR_DEV_POS_RANGE : 0;
+        } else {
+          page = t.table[(int64_t)b * t.ld_table + (pos >> c.shift)];
+          if (page < 0 || page >= c.n_pages) code = LR_DEV_PAGE_RANGE, page = -1;
+        }
+        if (code && t.err && (threadIdx.x & 63) == 0) *t.err = code;
+      }
+    }
+    if ((threadIdx.x & 63) == 0) at.pos[wave] = pos, at.page[wave] = page;
+  }
+  __syncthreads();
+}
+
+// The largest of a row's HD / 8 lanes, in all of them: exchanges within 16 lanes on the vector unit.
+template <int HD>
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, lr_dpp<0xb1>(v));    // quad_perm [1,0,3,2]
+  v = fmaxf(v, lr_dpp<0x4e>(v));    // quad_perm [2,3,0,1]
+  v = fmaxf(v, lr_dpp<0x141>(v));   // row_half_mirror: 8 lanes
+  if (HD == 128) v = fmaxf(v, lr_dpp<0x140>(v));   // row_mirror: 16 lanes
+  return v;
+}
+
+struct PagedWrite {
+  const u16* x;
+  int64_t ldx;
+  u16* q;
+  int64_t ldq;
+  const void* rope;
+  int rope_len, rot, rows, Hq, tokens;
+};
+
+// x[lo] c - x[hi] s and x[hi] c + x[lo] s for the 8 elements from d on, each product rounded by itself (as lr_rope_kv_write does it).
+// PAIRS: a pair is two neighbours; else element i and i + rot / 2, whose 8 are read besides.
+template <bool PAIRS, typename T>
+__device__ __forceinline__ void paged_turn(float* f, const u16* row, int d, const T* angles, int rot) {
+#pragma clang fp contract(off)
+  const int half = rot >> 1;
+  if constexpr (PAIRS) {
+    float t[8];
+    if constexpr (sizeof(T) == 2) {
+      unpack8(ld16(angles + d), t);
+    } else {
+      *reinterpret_cast<float4*>(t) = *reinterpret_cast<const float4*>(angles + d);
+      *reinterpret_cast<float4*>(t + 4) = *reinterpret_cast<const float4*>(angles + d + 4);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = f[2 * i], b = f[2 * i + 1], c = t[2 * i], s = t[2 * i + 1];
+      f[2 * i] = a * c - b * s;
+      f[2 * i + 1] = b * c + a * s;
+    }
+  } else {
+    const bool second = d >= half;
+    const int i0 = second ? d - half : d;
+    float o[8], t[16];
+    unpack8(ld16(row + (second ? d - half : d + half)), o);
+    if constexpr (sizeof(T) == 2) {
+      unpack8(ld16(angles + 2 * i0), t);
+      unpack8(ld16(angles + 2 * i0 + 8), t + 8);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(t + 4 * j) = *reinterpret_cast<const float4*>(angles + 2 * i0 + 4 * j);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float p = f[j] * t[2 * j], r = o[j] * t[2 * j + 1];
+      f[j] = second ? p + r : p - r;
+    }
+  }
+}
+
+template <int HD, bool E4M3, bool PAIRS, typename T>
+__global__ __launch_bounds__(256) void k_paged_write(const PagedCache c, const PagedBatch t, const PagedWrite w) {
+  __shared__ PagedPlace at;
+  const int row0 = blockIdx.x * w.tokens;
+  paged_places(c, t, row0, w.rows, w.tokens, w.rope ? w.rope_len : 0x7fffffff, at);
+  constexpr int LANES = HD / 8, ROWS = 256 / LANES;
+  const int heads = w.Hq + 2 * c.Hkv, d = threadIdx.x % LANES * 8;
+  for (int i = threadIdx.x / LANES; i < w.tokens * heads; i += ROWS) {   // (all lanes of a row go round together)
+    const int token = i / heads, head = i - token * heads, page = at.page[token];
+    if (page < 0) continue;
+    const int pos = at.pos[token];
+    const u16* const row = w.x + (row0 + token) * w.ldx + head * HD;
+    float f[8];
+    unpack8(ld16(row + d), f);
+    if (w.rope && head < w.Hq + c.Hkv && d < w.rot) paged_turn<PAIRS>(f, row, d, (const T*)w.rope + (int64_t)pos * w.rot, w.rot);
+    if (head < w.Hq) {
+      st16(w.q + (row0 + token) * w.ldq + head * HD + d, pack8(f));
+      continue;
+    }
+    const int value = head >= w.Hq + c.Hkv, kvh = head - w.Hq - value * c.Hkv, slot = pos & ((1 << c.shift) - 1);
+    u8* const to = (value ? c.v : c.k) + paged_offset<HD * (E4M3 ? 1 : 2)>(c, page, kvh);
+    if constexpr (!E4M3) {
+      st16(to + (slot * HD + d) * 2, pack8(f));
+    } else {
+      float amax = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(f[j]) < INFINITY ? fabsf(f[j]) : 0.0f);
+      amax = row_max<HD>(amax);
+      const u32 byte = paged_exponent(amax);
+      const float inv = paged_inverse(byte);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = fabsf(f[j]) < INFINITY ? f[j] * inv : NAN;   // (e4m3 has no infinities)
+      u32x2_t o;
+      o.x = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false), true);
+      o.y = __builtin_amdgcn_cvt_pk_fp8_f32(f[6], f[7], __builtin_amdgcn_cvt_pk_fp8_f32(f[4], f[5], 0, false), true);
+      *reinterpret_cast<u32x2_t*>(to + slot * HD + d) = o;
+      if (d == 0) c.scales[paged_scales(c, page, kvh) + (value << c.shift) + slot] = (u8)byte;
+    }
+  }
+}
+
+struct PagedRead {
+  u16 *k, *v;
+  int64_t ldk, ldv;
+  int rows, tokens;
+};
+
+template <int HD, bool E4M3>
+__global__ __launch_bounds__(256) void k_paged_read(const PagedCache c, const PagedBatch t, const PagedRead r) {
+  __shared__ PagedPlace at;
+  const int row0 = blockIdx.x * r.tokens;
+  paged_places(c, t, row0, r.rows, r.tokens, 0x7fffffff, at);
+  constexpr int LANES = HD / 8, ROWS = 256 / LANES;
+  const int d = threadIdx.x % LANES * 8;
+  for (int i = threadIdx.x / LANES; i < r.tokens * 2 * c.Hkv; i += ROWS) {
+    const int token = i / (2 * c.Hkv), j = i - token * 2 * c.Hkv, value = j >= c.Hkv, kvh = j - value * c.Hkv, page = at.page[token];
+    if (page < 0) continue;
+    const int slot = at.pos[token] & ((1 << c.shift) - 1);
+    const u8* const from = (value ? c.v : c.k) + paged_offset<HD * (E4M3 ? 1 : 2)>(c, page, kvh);
+    uint4 o;
+    if constexpr (!E4M3) {
+      o = ld16(from + (slot * HD + d) * 2);
+    } else {
+      const u32x2_t raw = *reinterpret_cast<const u32x2_t*>(from + slot * HD + d);
+      const float s = paged_scale(c.scales[paged_scales(c, page, kvh) + (value << c.shift) + slot]);
+      o.x = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.x, s, false));
+      o.y = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.x, s, true));
+      o.z = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.y, s, false));
+      o.w = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.y, s, true));
+    }
+    st16((value ? r.v + (row0 + token) * r.ldv : r.k + (row0 + token) * r.ldk) + kvh * HD + d, o);
+  }
+}
+
+// Tokens of a workgroup: as many as give every lane something, the grid no fewer workgroups than the chip holds at once.
+static inline int paged_tokens(int rows, int heads, int hd) {
+  const int fill = 256 / (hd / 8) / heads, spread = rows / (8 * 256);
+  const int n = fill > spread ? spread : fill;
+  return n < 1 ? 1 : n > PAGED_TOKENS ? PAGED_TOKENS : n;
+}
+
+template <int HD, bool E4M3, bool PAIRS>
+static void launch_write(bool f32, unsigned grid, const PagedCache& c, const PagedBatch& t, const PagedWrite& w, hipStream_t s) {
+  if (f32) k_paged_write<HD, E4M3, PAIRS, float><<<dim3(grid), dim3(256), 0, s>>>(c, t, w);
+  else k_paged_write<HD, E4M3, PAIRS, u16><<<dim3(grid), dim3(256), 0, s>>>(c, t, w);
+}
+
+extern "C" int lr_paged_write(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, const void* qkv, int64_t ldqkv, void* q, int64_t ldq,
+                              int rows, int Hq, const void* rope, int rope_len, int rot, int interleaved, int rope_dtype, lr_stream_t stream) {
+  PagedCache c;
+  PagedBatch t;
+  if (const int rc = paged_arguments(cache, batch, c, t)) return rc;
+  LR_REQUIRE_PTR(qkv);
+  LR_REQUIRE_PTR(q);
+  LR_OPTIONAL_PTR(rope);
+  const int hd = cache->head_dim;
+  if (rows <= 0 || Hq <= 0 || Hq % c.Hkv || (t.starts == nullptr && rows != t.B)) return LR_E_SHAPE;
+  if (Hq > 65535 / 3 || ldqkv < (int64_t)(Hq + 2 * c.Hkv) * hd || ldq < (int64_t)Hq * hd) return LR_E_SHAPE;
+  if (ldqkv % 8 || ldq % 8) return LR_E_ALIGN;
+  if (rope && (rope_len <= 0 || rot <= 0 || rot > hd)) return LR_E_SHAPE;
+  if (rope && (rot % 16 || (rope_dtype != LR_BF16 && rope_dtype != LR_F32))) return LR_E_UNSUPPORTED;
+  const int tokens = paged_tokens(rows, Hq + 2 * c.Hkv, hd);
+  const PagedWrite w = {(const u16*)qkv, ldqkv, (u16*)q, ldq, rope, rope_len, rot, rows, Hq, tokens};
+  const unsigned grid = (unsigned)((rows + tokens - 1) / tokens);
+  const bool f32 = rope_dtype == LR_F32;
+  hipStream_t s = (hipStream_t)stream;
+  const bool e4m3 = cache->format == LR_CACHE_E4M3;
+#define LR_WRITE(HDV, E, P) \
+  if (hd == HDV && e4m3 == E && (interleaved != 0) == P) launch_write<HDV, E, P>(f32, grid, c, t, w, s);
+  LR_WRITE(64, false, false) LR_WRITE(64, false, true) LR_WRITE(64, true, false) LR_WRITE(64, true, true)
+  LR_WRITE(128, false, false) LR_WRITE(128, false, true) LR_WRITE(128, true, false) LR_WRITE(128, true, true)
+#undef LR_WRITE
+  return lr_launch_status();
+}
+
+extern "C" int lr_paged_read(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, void* k, int64_t ldk, void* v, int64_t ldv, int rows,
+                             lr_stream_t stream) {
+  PagedCache c;
+  PagedBatch t;
+  if (const int rc = paged_arguments(cache, batch, c, t)) return rc;
+  LR_REQUIRE_PTR(k);
+  LR_REQUIRE_PTR(v);
+  const int hd = cache->head_dim;
+  if (rows <= 0 || (t.starts == nullptr && rows != t.B) || c.Hkv > 65535) return LR_E_SHAPE;
+  if (ldk < (int64_t)c.Hkv * hd || ldv < (int64_t)c.Hkv * hd) return LR_E_SHAPE;
+  if (ldk % 8 || ldv % 8) return LR_E_ALIGN;
+  const int tokens = paged_tokens(rows, 2 * c.Hkv, hd);
+  const PagedRead r = {(u16*)k, (u16*)v, ldk, ldv, rows, tokens};
+  const dim3 grid((unsigned)((rows + tokens - 1) / tokens));
+  hipStream_t s = (hipStream_t)stream;
+  const bool e4m3 = cache->format == LR_CACHE_E4M3;
+  if (hd == 128 && e4m3) k_paged_read<128, true><<<grid, dim3(256), 0, s>>>(c, t, r);
+  else if (hd == 128) k_paged_read<128, false><<<grid, dim3(256), 0, s>>>(c, t, r);
+  else if (e4m3) k_paged_read<64, true><<<grid, dim3(256), 0, s>>>(c, t, r);
+  else k_paged_read<64, false><<<grid, dim3(256), 0, s>>>(c, t, r);
+  return lr_launch_status();
+}

@@ -144,6 +144,12 @@ _PROTOS = {
     "lr_moe_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "lr_moe": (c_int, [c_void_p, c_void_p]),
     "lr_linear_multi_route": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p]),
+    "lr_paged_write": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int,
+                               c_void_p]),
+    "lr_paged_read": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p]),
+    "lr_paged_attention_scratch_bytes": (c_size_t, [c_void_p, c_void_p, c_int, c_int]),
+    "lr_paged_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_float, c_void_p, c_size_t,
+                                   c_void_p]),
 }
 
 
@@ -748,9 +754,10 @@ def device_error_word(device) -> torch.Tensor:
 
 
 _ERR_WORDS = {}
-DEV_WAIT_EXPIRED, DEV_POS_RANGE = 1, 2
+DEV_WAIT_EXPIRED, DEV_POS_RANGE, DEV_PAGE_RANGE = 1, 2, 3
 _DEV_ERR_TEXT = {DEV_WAIT_EXPIRED: "a bounded cross-workgroup wait of the decode-step kernel expired",
-                 DEV_POS_RANGE: "a position outside the KV cache or the RoPE table was used"}
+                 DEV_POS_RANGE: "a position outside the KV cache or the RoPE table was used",
+                 DEV_PAGE_RANGE: "a page number outside the paged KV cache was used"}
 
 
 def raise_on_device_error(device=None, fused_steps=()):
@@ -1366,6 +1373,108 @@ def linear_multi_route(desc, *projections):
 def moe(desc):
     """The experts' rows of `desc` (lr_moe), routed first unless linear_multi_route has done so."""
     _check(load().lr_moe(ctypes.byref(desc), _stream()), "lr_moe")
+
+
+class _PagedCache(ctypes.Structure):   # lr_paged_cache_t
+    _fields_ = [(n, c_void_p) for n in ("k", "v", "scales")] + \
+               [(n, c_int32) for n in ("n_pages", "page", "n_kv_head", "head_dim", "format")]
+
+
+class _PagedBatch(ctypes.Structure):   # lr_paged_batch_t
+    _fields_ = [("table", c_void_p), ("ld_table", c_int64), ("lengths", c_void_p), ("starts", c_void_p), ("err", c_void_p),
+                ("B", c_int32), ("pages", c_int32)]
+
+
+CACHE_BF16, CACHE_E4M3 = 0, 1
+
+
+def paged_cache_desc(k, v, scales=None) -> _PagedCache:
+    """k, v [n_pages, kv heads, page, head_dim] bf16, or float8_e4m3fn with scales [n_pages, kv heads, 2, page] uint8."""
+    e4m3 = k.dtype == torch.float8_e4m3fn
+    dtype = k.dtype if e4m3 else torch.bfloat16
+    assert k.dim() == 4 and k.shape == v.shape and k.is_contiguous() and v.is_contiguous(), "k and v: dense pages of the same shape"
+    assert e4m3 == (scales is not None), "scales go with e4m3 pages, and only with them"
+    n, heads, page, hd = k.shape
+    if e4m3:
+        assert tuple(scales.shape) == (n, heads, 2, page) and scales.is_contiguous() and scales.device == k.device
+    assert v.device == k.device
+    return _PagedCache(_dev(k, dtype), _dev(v, dtype), _dev(scales, torch.uint8) if e4m3 else None, n, page, heads, hd,
+                       CACHE_E4M3 if e4m3 else CACHE_BF16)
+
+
+def paged_batch_desc(table, lengths, starts=None) -> _PagedBatch:
+    """table [B, pages], lengths [B], starts [B + 1] or None: int32 on the device."""
+    B, pages = table.shape
+    assert table.stride(1) == 1 or pages == 1
+    assert tuple(lengths.shape) == (B,) and lengths.is_contiguous() and lengths.device == table.device
+    if starts is not None:
+        assert tuple(starts.shape) == (B + 1,) and starts.is_contiguous() and starts.device == table.device
+    i = torch.int32
+    return _PagedBatch(_dev(table, i), max(table.stride(0), pages), _dev(lengths, i), None if starts is None else _dev(starts, i),
+                       device_error_word(table.device).data_ptr(), B, pages)
+
+
+def _paged_rows(t, width, device):
+    """(address, row stride, rows) of a [rows, width] bf16 matrix with dense rows."""
+    rows, cols = t.shape
+    ld, unit = t.stride()
+    if t.dtype != torch.bfloat16 or cols != width or unit != 1 or t.device != device:
+        raise ValueError(f"expected [rows, {width}] bfloat16 with dense rows on {device}, got {tuple(t.shape)} {t.dtype} "
+                         f"with strides {t.stride()} on {t.device}")
+    return t.data_ptr(), (ld if rows > 1 else cols), rows
+
+
+def _paged_stream(device) -> int:
+    """The current stream, which has to be one of the device that the cache is on."""
+    s = torch.cuda.current_stream()
+    if s.device != device:
+        raise ValueError(f"the cache is on {device}, the current stream on {s.device}")
+    return s.cuda_stream
+
+
+def paged_write(cache, batch, qkv, q, n_head, device, rope=None, interleaved=True):
+    """lr_paged_write: qkv [rows, (n_head + 2 kv heads) head_dim], q [rows, n_head head_dim]; rope [positions, rot / 2, 2] bf16 or fp32."""
+    hd = cache.head_dim
+    x, ldx, rows = _paged_rows(qkv, (n_head + 2 * cache.n_kv_head) * hd, device)
+    o, ldo, n = _paged_rows(q, n_head * hd, device)
+    if n != rows:
+        raise ValueError(f"{rows} rows of qkv, {n} of q")
+    r, length, rot, f32 = None, 0, 0, 0
+    if rope is not None:
+        length, rot = rope.shape[0], 2 * rope.shape[1]
+        if rope.dim() != 3 or rope.shape[2] != 2 or not rope.is_contiguous() or rope.device != device or \
+                rope.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError(f"rope is dense [positions, rot / 2, 2], bfloat16 or float32, on {device}")
+        r, f32 = rope.data_ptr(), int(rope.dtype == torch.float32)
+    _check(load().lr_paged_write(ctypes.byref(cache), ctypes.byref(batch), x, ldx, o, ldo, rows, n_head, r, length, rot, int(interleaved), f32,
+                                 _paged_stream(device)), "lr_paged_write")
+    return q
+
+
+def paged_read(cache, batch, k, v, device):
+    """lr_paged_read: k, v [rows, kv heads * head_dim]."""
+    a, lda, rows = _paged_rows(k, cache.n_kv_head * cache.head_dim, device)
+    b, ldb, n = _paged_rows(v, cache.n_kv_head * cache.head_dim, device)
+    if n != rows:
+        raise ValueError(f"{rows} rows of k, {n} of v")
+    _check(load().lr_paged_read(ctypes.byref(cache), ctypes.byref(batch), a, lda, b, ldb, rows, _paged_stream(device)), "lr_paged_read")
+    return k, v
+
+
+def paged_attention_scratch_bytes(cache, batch, rows, n_head) -> int:
+    return int(load().lr_paged_attention_scratch_bytes(ctypes.byref(cache), ctypes.byref(batch), rows, n_head))
+
+
+def paged_attention(cache, batch, q, y, n_head, device, scratch, scale=None):
+    """lr_paged_attention: q, y [rows, n_head * head_dim]; scratch uint8, zero before the first call."""
+    x, ldx, rows = _paged_rows(q, n_head * cache.head_dim, device)
+    o, ldo, n = _paged_rows(y, n_head * cache.head_dim, device)
+    if n != rows:
+        raise ValueError(f"{rows} rows of q, {n} of y")
+    _check(load().lr_paged_attention(ctypes.byref(cache), ctypes.byref(batch), x, ldx, o, ldo, rows, n_head,
+                                     cache.head_dim ** -0.5 if scale is None else scale, scratch.data_ptr(), scratch.numel(),
+                                     _paged_stream(device)), "lr_paged_attention")
+    return y
 
 
 def _ladder_model_desc(model, attention_workgroups: int = 0):

@@ -58,6 +58,95 @@ class KVCache(nn.Module):
         return self.k_cache, self.v_cache
 
 
+class PagedBatch:
+    """Sequences of one call on paged caches of one shape (PagedKVCache.batch): table, lengths and starts on the device, and the
+    scratch of the attention.  The tensors may be written between calls, also between replays of a captured graph; calls that may overlap
+    have batches of their own."""
+
+    def __init__(self, cache: "PagedKVCache", table: Tensor, lengths: Tensor, n_head: int, starts: Optional[Tensor], rows: int):
+        self.table, self.lengths, self.starts, self.n_head, self.rows = table, lengths, starts, n_head, rows
+        self.shape = cache.shape
+        self.desc = _hip.paged_batch_desc(table, lengths, starts)
+        need = _hip.paged_attention_scratch_bytes(cache.desc(), self.desc, rows, n_head)
+        if need == 0:
+            raise _hip.LadderHipError(f"a paged cache of pages {cache.shape} is not served with {n_head} q heads and a table "
+                                      f"{tuple(table.shape)}: head_dim 64 or 128, pages of 16 to 256 tokens (a power of two)")
+        self.scratch = torch.zeros(need, dtype=torch.uint8, device=table.device)
+
+
+class PagedKVCache(nn.Module):
+    """Keys and values of sequences of any lengths, by pages of `page` tokens: k_pages, v_pages [n_pages, kv heads of this rank, page,
+    head_dim], bf16 or float8_e4m3fn (quantised as they are written, a power of two per row in `scales`).  Beside KVCache, whose
+    sequences share one position and have max_seq_length slots each.  Which page belongs to whom is the caller's: a batch() carries
+    the tables.  One launch each: write() rotates q and k and stores k and v, attend() is the attention of the call's rows, read() gives
+    the call's tokens back (lr_paged_write, lr_paged_attention, lr_paged_read)."""
+
+    def __init__(self, n_pages: int, page: int, n_heads: int, head_dim: int, dtype=torch.bfloat16, device=None):
+        super().__init__()
+        assert dtype in (torch.bfloat16, torch.float8_e4m3fn), f"pages are bfloat16 or float8_e4m3fn, not {dtype}"
+        zeros = lambda *s, t: torch.zeros(s, dtype=t, device=device)
+        self._hold(zeros(n_pages, n_heads, page, head_dim, t=dtype), zeros(n_pages, n_heads, page, head_dim, t=dtype),
+                   zeros(n_pages, n_heads, 2, page, t=torch.uint8) if dtype == torch.float8_e4m3fn else None)
+
+    @classmethod
+    def from_pages(cls, k_pages: Tensor, v_pages: Tensor, scales: Optional[Tensor] = None) -> "PagedKVCache":
+        """A cache on memory that is there already."""
+        self = cls.__new__(cls)
+        nn.Module.__init__(self)
+        self._hold(k_pages, v_pages, scales)
+        return self
+
+    def _hold(self, k, v, scales):
+        self.register_buffer("k_pages", k)
+        self.register_buffer("v_pages", v)
+        self.register_buffer("scales", scales)
+        self._desc = None
+
+    @property
+    def shape(self):
+        return tuple(self.k_pages.shape[1:])
+
+    def desc(self):
+        if self._desc is None:
+            self._desc = _hip.paged_cache_desc(self.k_pages, self.v_pages, self.scales)
+            self._device = self.k_pages.device
+        return self._desc
+
+    def _apply(self, fn, recurse=True):
+        """Moving the module moves the pages (.to(device), .cuda()); their types stay what they are."""
+        kept = fn
+        fn = lambda t: kept(t).to(t.dtype) if t.dtype in (torch.bfloat16, torch.float8_e4m3fn) else kept(t)
+        self._desc = None
+        return super()._apply(fn, recurse)
+
+    def batch(self, table: Tensor, lengths: Tensor, n_head: int, starts: Optional[Tensor] = None, rows: Optional[int] = None) -> PagedBatch:
+        """table [B, pages], lengths [B] (the call's own tokens among them), starts [B + 1] int32 on the device (None: one row per
+        sequence); `rows`: how many rows a call has at most (given with starts).  Serves every cache of the same shape."""
+        assert starts is None or rows is not None, "with starts, say how many rows a call has at most"
+        assert starts is not None or rows in (None, table.shape[0]), "without starts there is one row per sequence"
+        return PagedBatch(self, table, lengths, n_head, starts, table.shape[0] if rows is None else rows)
+
+    def _check(self, batch: PagedBatch, rows: int):
+        desc = self.desc()
+        if batch.shape != self.shape or rows > batch.rows:
+            raise ValueError(f"a batch for up to {batch.rows} rows and pages {batch.shape}: got {rows} rows, pages {self.shape}")
+        return desc
+
+    def write(self, batch: PagedBatch, qkv: Tensor, q: Tensor, rope: Optional[Tensor] = None, interleaved: bool = True) -> Tensor:
+        """qkv [rows, (n_head + 2 kv heads) head_dim] fresh from the fused projection: q and k rotated by rope [positions, rot / 2, 2]
+        (precompute_freqs_cis's table, or fp32; pairs of neighbours, or of the two halves of the first rot dimensions), q to `q` (which may
+        be qkv's own columns), k and v into the pages."""
+        return _hip.paged_write(self._check(batch, qkv.shape[0]), batch.desc, qkv, q, batch.n_head, self._device, rope, interleaved)
+
+    def read(self, batch: PagedBatch, k: Tensor, v: Tensor):
+        """The call's tokens back, [rows, kv heads * head_dim] bf16."""
+        return _hip.paged_read(self._check(batch, k.shape[0]), batch.desc, k, v, self._device)
+
+    def attend(self, batch: PagedBatch, q: Tensor, y: Tensor, scale: Optional[float] = None) -> Tensor:
+        """y [rows, n_head * head_dim] = attention of the rotated q's rows, each on its sequence's keys up to its own position."""
+        return _hip.paged_attention(self._check(batch, q.shape[0]), batch.desc, q, y, batch.n_head, self._device, batch.scratch, scale)
+
+
 class RMSNorm(nn.Module):
     def __init__(self, dim: int, eps: float = 1e-5):
         super().__init__()

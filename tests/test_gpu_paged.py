@@ -1,0 +1,535 @@
+"""The kernels of the paged key-value cache against their restatement in float64 (bits where the definition gives them).
+
+What no sequence has in the pages is NaN, with the largest scale where rows have one; lengths lie around the edges of tiles and pages."""
+import math
+
+import pytest
+import torch
+
+from oracle import paged_oracle as O
+from paged_cases import BF, E4M3, F32, F64, Case, bound
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+
+
+@pytest.fixture(scope="module")
+def hip():
+    from gpt_fast import _hip
+
+    _hip.load()
+    return _hip
+
+
+@pytest.fixture(autouse=True)
+def _no_device_error():
+    from gpt_fast import _hip
+
+    yield
+    _hip.raise_on_device_error()
+
+
+def rnd(*shape, seed=0, scale=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(BF)
+
+
+def bits(t):
+    return t.cpu().contiguous().view(torch.uint8)
+
+
+# ------------------------------------------------------------------------------------------------ write
+
+def written(case, hq, rope, rot, interleaved, qkv, dtype=F32):
+    """(q, {(page, slot): (k, v)}) in `dtype` of the rows that have a place."""
+    hkv, hd = case.hkv, case.hd
+    q, rows = {}, {}
+    for r, _, pos, page, slot in O.places(case.table, case.lengths, case.starts, case.page):
+        x = qkv[r].view(hq + 2 * hkv, hd).to(dtype)
+        if rope is not None:
+            x = torch.cat([O.turn(x[:hq + hkv], rope[pos], rot, interleaved, dtype), x[hq + hkv:]])
+        q[r], rows[page, slot] = x[:hq], (x[hq:hq + hkv], x[hq + hkv:])
+    return q, rows
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("hq,hkv,hd,page,rot,table,lengths,new", [
+    (8, 1, 128, 16, 128, BF, [17], None),                                # a rank shard's decode step
+    (4, 2, 64, 32, 32, F32, [1, 0, 33, 64, 31], None),                   # empty places, first and last slots of pages
+    (3, 3, 64, 16, 64, F32, [5, 40, 16, 16], [5, 3, 0, 16]),             # prompts, a portion, a sequence without rows
+    (14, 2, 64, 256, 16, BF, [300, 2], [299, 2]),
+    (2, 1, 128, 64, None, BF, [70, 64], [70, 1]),                        # nothing turned
+    (16, 8, 128, 128, 64, F32, [129] + [3] * 69, None),                  # more sequences than a wave has lanes
+])
+def test_write(hip, e4m3, interleaved, hq, hkv, hd, page, rot, table, lengths, new):
+    case = Case(lengths, hkv, hd, page, e4m3, seed=3, new=new)
+    cache, batch = case.on(DEV, hq, rows=case.rows + 3)
+    width = (hq + 2 * hkv) * hd
+    behind = 0 if new is None else 3
+    buf = rnd(case.rows + behind, width + 24, seed=4)
+    buf[0, hq * hd:hq * hd + 8] *= 100.0
+    qkv = buf[:, 8:8 + width]
+    rope = None
+    if rot:
+        g = torch.Generator().manual_seed(5)
+        angle = torch.rand(max(lengths), rot // 2, generator=g) * 6.28
+        rope = torch.stack([angle.cos(), angle.sin()], -1).to(table)
+    k0, v0 = case.k.clone(), case.v.clone()
+    s0 = None if case.scales is None else case.scales.clone()
+    dev = buf.to(DEV)
+    q = torch.full((case.rows + behind, hq * hd + 8), 7.0, dtype=BF, device=DEV)
+    cache.write(batch, dev[:, 8:8 + width], q[:, :hq * hd], None if rope is None else rope.to(DEV), interleaved)
+    assert torch.equal(bits(dev), bits(buf)), "qkv is read only"
+    want_q, rows = written(case, hq, rope, rot, interleaved, qkv)
+    exact_q, exact_rows = written(case, hq, rope, rot, interleaved, qkv, F64)
+    expect = torch.full(q.shape, 7.0, dtype=BF)
+    for r, x in want_q.items():
+        expect[r, :hq * hd] = x.reshape(-1).to(BF)
+        # against 64 bits: half a step of bf16, and 2^-24 of each product and the sum (products of at most |x| each)
+        near = 2.0 ** -8 * exact_q[r].abs() + 4 * 2.0 ** -24 * qkv[r].view(-1, hd)[:hq].double().abs().amax(-1, keepdim=True)
+        assert ((q[r, :hq * hd].cpu().double().view(hq, hd) - exact_q[r]).abs() <= near).all()
+    assert torch.equal(bits(q), bits(expect)), "q, and nothing besides"
+    for (p, slot), kv in rows.items():
+        for which, pages in enumerate((k0, v0)):
+            if e4m3:
+                pages[p, :, slot], s0[p, :, which, slot] = O.quantise(kv[which])
+            else:
+                pages[p, :, slot] = kv[which].to(BF)
+    assert torch.equal(bits(cache.k_pages), bits(k0)) and torch.equal(bits(cache.v_pages), bits(v0)), "pages: these rows, nothing besides"
+    if e4m3:
+        assert torch.equal(cache.scales.cpu(), s0)
+        for (p, slot), kv in exact_rows.items():
+            got = O.values(cache.k_pages[p:p + 1, :, slot:slot + 1].cpu(), cache.scales[p:p + 1, :, :, slot:slot + 1].cpu())[0, :, 0]
+            step = torch.exp2(s0[p, :, 0, slot].double() - 127)[:, None]
+            near = torch.maximum(2.0 ** -4 * kv[0].abs(), 2.0 ** -10 * step) * (1 + 2.0 ** -20) + 2.0 ** -20 * step
+            assert ((got - kv[0]).abs() <= near).all()
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_write_in_place_gives_the_same_bits(hip, interleaved):
+    hq, hkv, hd = 6, 2, 128
+    case = Case([40, 21], hkv, hd, 16, False, new=[17, 21])
+    cache, batch = case.on(DEV, hq)
+    other, _ = case.on(DEV, hq)
+    qkv = rnd(case.rows, (hq + 2 * hkv) * hd, seed=1).to(DEV)
+    rope = torch.randn(64, hd // 2, 2, generator=torch.Generator().manual_seed(2)).to(DEV)
+    q = torch.empty(case.rows, hq * hd, dtype=BF, device=DEV)
+    cache.write(batch, qkv, q, rope, interleaved)
+    mine = qkv.clone()
+    other.write(batch, mine, mine[:, :hq * hd], rope, interleaved)
+    assert torch.equal(bits(mine[:, :hq * hd]), bits(q)) and torch.equal(mine[:, hq * hd:], qkv[:, hq * hd:])
+    assert torch.equal(bits(other.k_pages), bits(cache.k_pages)) and torch.equal(bits(other.v_pages), bits(cache.v_pages))
+
+
+def test_write_of_values_that_are_not_finite_or_far_apart(hip):
+    """Rows of zeros, with infinities and NaN, of the smallest and the largest numbers."""
+    hq, hkv, hd = 1, 1, 64
+    n = 9
+    case = Case([n], hkv, hd, 16, True, new=[n])
+    cache, batch = case.on(DEV, hq)
+    qkv = rnd(n, 3 * hd, seed=1)
+    k = qkv[:, hd:2 * hd]
+    k[0] = 0
+    k[1, 3], k[1, 60] = math.inf, -math.inf
+    k[2, 5] = math.nan
+    k[3] = math.nan
+    k[4] *= 1e-38
+    k[5] *= 3e37
+    k[6] = 448.0
+    k[7, 0] = 452.0          # the exponent is one larger: 226
+    k[8] = torch.logspace(-6, 2, hd).to(BF)
+    cache.write(batch, qkv.to(DEV), torch.empty(n, hd, dtype=BF, device=DEV))
+    page = int(case.table[0, 0])
+    for which, pages in enumerate((cache.k_pages, cache.v_pages)):
+        want, byte = O.quantise(qkv[:, (1 + which) * hd:(2 + which) * hd].float())
+        got = pages[page, 0, :n].cpu()
+        assert torch.equal(cache.scales[page, 0, which, :n].cpu(), byte)
+        assert torch.equal(got.float().isnan(), want.float().isnan())
+        assert torch.equal(torch.nan_to_num(got.float()), torch.nan_to_num(want.float()))
+
+
+def test_rows_and_pages_out_of_range_are_left_alone(hip):
+    hq, hkv, hd, page = 2, 1, 64, 16
+    case = Case([20, 20, 20, 20], hkv, hd, page, False, new=[2, 2, 2, 2])
+    cache, batch = case.on(DEV, hq)
+    batch.table[0, 1] = -1                     # both rows of sequence 0
+    batch.table[1, 1] = case.n_pages           # and of 1
+    batch.lengths[2] = 1                       # its first row would be at position -1
+    batch.lengths[3] = case.table.shape[1] * page + 1     # its last row has no page in the table
+    table, lengths = batch.table.cpu(), batch.lengths.tolist()
+    table[3, 2:] = table[3, 0]
+    batch.table[3, 2:] = table[3, 0]
+    qkv = rnd(8, 4 * hd, seed=2)
+    q = torch.full((8, hq * hd), 5.0, dtype=BF, device=DEV)
+    k0 = cache.k_pages.clone()
+    cache.write(batch, qkv.to(DEV), q)
+    with pytest.raises(hip.LadderHipError, match="outside"):
+        hip.raise_on_device_error(DEV)
+    there = [(r, p, s) for r, b, pos, p, s in O.places(table, lengths, case.starts, page) if 0 <= p < case.n_pages]
+    assert [t[0] for t in there] == [5, 6]
+    want_q, want_k = torch.full((8, hq * hd), 5.0, dtype=BF), k0.cpu()
+    for r, p, s in there:
+        want_q[r], want_k[p, :, s] = qkv[r, :hq * hd], qkv[r, hq * hd:(hq + 1) * hd].view(1, hd)
+    assert torch.equal(bits(q), bits(want_q)) and torch.equal(bits(cache.k_pages), bits(want_k))
+    # read back: the same two rows
+    a, b = (torch.full((8, hd), 9.0, dtype=BF, device=DEV) for _ in range(2))
+    cache.read(batch, a, b)
+    with pytest.raises(hip.LadderHipError, match="outside"):
+        hip.raise_on_device_error(DEV)
+    assert [r for r in range(8) if not (a[r] == 9).all()] == [5, 6]
+    # positions without an angle
+    case = Case([9], hkv, hd, page, False)
+    cache, batch = case.on(DEV, hq)
+    q.fill_(5.0)
+    cache.write(batch, qkv[:1].to(DEV), q[:1], torch.ones(8, hd // 2, 2, device=DEV))
+    with pytest.raises(hip.LadderHipError, match="position"):
+        hip.raise_on_device_error(DEV)
+    assert (q == 5).all()
+
+
+# ------------------------------------------------------------------------------------------------ read
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("hkv,hd,page,lengths,new", [
+    (1, 128, 16, [1], None), (2, 64, 32, [33, 0, 32, 5], None), (8, 128, 64, [130, 64, 1], [130, 64, 1]), (3, 64, 16, [50, 7], [20, 0]),
+    (1, 64, 256, [1] * 130, [1] * 130), (24, 128, 128, [300], [300]),
+])
+def test_read(hip, e4m3, hkv, hd, page, lengths, new):
+    case = Case(lengths, hkv, hd, page, e4m3, seed=6, new=new)
+    cache, batch = case.on(DEV, hkv, rows=case.rows + 2)
+    n = case.rows + (0 if new is None else 2)
+    k, v = (torch.full((n, hkv * hd + 8 * i), 3.0, dtype=BF, device=DEV) for i in (1, 2))
+    cache.read(batch, k[:, :hkv * hd], v[:, :hkv * hd])
+    for which, got in enumerate((k, v)):
+        want = torch.full(got.shape, 3.0, dtype=BF)
+        x = O.values((case.k, case.v)[which], case.scales, which)
+        for r, _, _, p, slot in O.places(case.table, case.lengths, case.starts, page):
+            want[r, :hkv * hd] = x[p, :, slot].reshape(-1).to(BF)       # (exact)
+        assert torch.equal(bits(got), bits(want))
+
+
+# ------------------------------------------------------------------------------------------------ attention
+
+WEIGHT = 2.0 ** -16     # decode: a weight enters as two bf16 numbers; prompts see the tests below
+
+
+def attend(case, hq, seed=11, scale=None, q_scale=1.0, weight=WEIGHT, behind=0, pad=8):
+    cache, batch = case.on(DEV, hq, rows=None if case.starts is None else case.rows + behind)
+    q = rnd(case.rows + behind, hq * case.hd, seed=seed, scale=q_scale)
+    buf = torch.full((q.shape[0], hq * case.hd + pad), 3.0, dtype=BF, device=DEV)
+    src = torch.full((q.shape[0], hq * case.hd + 2 * pad), 3.0, dtype=BF, device=DEV)
+    src[:, pad:pad + q.shape[1]] = q.to(DEV)
+    cache.attend(batch, src[:, pad:pad + q.shape[1]], buf[:, :q.shape[1]], scale)
+    got = buf.cpu()
+    assert (got[:, q.shape[1]:] == 3).all()
+    y, spread, size = case.oracle(q, hq, scale)
+    got = got[:, :q.shape[1]].double().view(y.shape)
+    rows = ~y.isnan().all(-1).all(-1)
+    assert (got[~rows] == 3).all(), "rows behind the last sequence are left as they were"
+    near = bound(y, spread, size, max(case.lengths + [1]), case.hd, weight)
+    off = ((got - y).abs() / near)[rows]
+    assert not off.isnan().any() and (off.numel() == 0 or off.max() <= 1), f"{off.max():.2f} of what rounding explains"
+    return cache, batch, q, got
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 1, 128), (1, 1, 64), (6, 2, 128), (14, 2, 64), (16, 1, 128), (3, 3, 64), (40, 2, 64), (17, 1, 128)])
+@pytest.mark.parametrize("page,lengths", [(16, [1, 0, 15, 16, 17, 33]), (64, [128, 31, 32, 0, 257, 63]), (256, [513, 255])])
+def test_decode(hip, e4m3, hq, hkv, hd, page, lengths):
+    attend(Case(lengths, hkv, hd, page, e4m3, seed=hq + page), hq)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lengths,hq,hkv,hd,page", [
+    ([9001], 4, 1, 128, 16), ([5000, 1, 0, 700], 2, 2, 64, 32), ([33] * 300, 2, 1, 64, 16), ([0] * 70 + [100], 4, 4, 128, 64),
+    ([2049, 4095], 8, 1, 128, 128), ([0, 0], 8, 1, 128, 16),
+])
+def test_decode_of_long_and_of_many_sequences(hip, e4m3, lengths, hq, hkv, hd, page):
+    attend(Case(lengths, hkv, hd, page, e4m3, seed=5), hq)
+
+
+PROMPT = 2.0 ** -8      # prompts: a weight enters as one bf16 number
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("hq,hkv,hd,page,lengths,new", [
+    (8, 1, 128, 16, [1], [1]), (4, 1, 64, 32, [33, 5], [33, 5]), (2, 2, 128, 64, [200, 64, 65], [70, 0, 65]),
+    (6, 2, 64, 16, [31, 32, 33, 0, 1], [31, 32, 33, 0, 1]), (12, 4, 128, 256, [300, 17], [40, 17]), (5, 1, 64, 16, [90, 250], [90, 129]),
+    (16, 1, 128, 128, [700], [3]), (1, 1, 128, 16, [64] * 70, [1, 2] * 35), (32, 8, 64, 16, [100, 77], [100, 77]),
+    (8, 1, 128, 32, [3000], [65]), (4, 4, 64, 64, [0, 0, 2], [0, 0, 2]), (7, 1, 128, 16, [150], [150]),
+])
+def test_prompts(hip, e4m3, hq, hkv, hd, page, lengths, new):
+    attend(Case(lengths, hkv, hd, page, e4m3, seed=7, new=new), hq, weight=PROMPT, behind=3)
+
+
+def test_rows_ahead_of_a_sequences_first_token_see_nothing(hip):
+    """More rows than tokens: those at negative positions are zeros."""
+    for e4m3 in (False, True):
+        case = Case([3, 40], 1, 64, 16, e4m3, new=[5, 2])
+        *_, got = attend(case, 2, weight=PROMPT)
+        assert (got[:2] == 0).all() and (got[2] != 0).any()
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("new", [None, [40, 17]])
+def test_scores_far_apart(hip, e4m3, new):
+    """Scores of some hundreds, of both signs; a scale of one's own."""
+    attend(Case([500, 77], 1, 128, 16, e4m3, seed=8, new=new, spread=4.0), 4, q_scale=6.0, weight=PROMPT if new else WEIGHT)
+    attend(Case([500, 77], 1, 64, 16, e4m3, seed=9, new=new), 4, scale=1e-3, weight=PROMPT if new else WEIGHT)
+    attend(Case([500, 77], 1, 64, 16, e4m3, seed=9, new=new), 4, scale=1.0, weight=PROMPT if new else WEIGHT)
+
+
+@pytest.mark.parametrize("new", [None, [2, 30]])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_one_key_that_stands_out(hip, e4m3, new):
+    """The winning key first, last, at a tile's or a page's edge: the output is its value, whatever stood before and after."""
+    hq, hkv, hd, page = 2, 1, 128, 16
+    n = 300
+    for at in (0, 15, 16, 31, 32, 127, 128, 255, 269 if new else 299):
+        case = Case([5, n], hkv, hd, page, e4m3, seed=at, new=new)
+        k = torch.zeros(hd)
+        k[7] = 256.0
+        p, slot = int(case.table[1, at // page]), at % page
+        case.k[p, 0, slot] = (k / 64.0 if e4m3 else k).to(case.k.dtype)
+        if e4m3:
+            case.scales[p, 0, 0, slot] = 127 + 6
+        cache, batch = case.on(DEV, hq)
+        q = torch.zeros(case.rows, hq * hd, dtype=BF)
+        q[:, 7::hd] = 64.0
+        y = torch.empty(case.rows, hq * hd, dtype=BF, device=DEV)
+        cache.attend(batch, q.to(DEV), y)
+        want = O.values(case.v, case.scales, 1)[p, 0, slot].to(BF)
+        assert torch.equal(y[-1].cpu(), want.repeat(hq)), at
+
+
+@pytest.mark.parametrize("new", [None, [1, 20]])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_pages_out_of_range_are_not_there(hip, e4m3, new):
+    case = Case([40, 70], 2, 64, 16, e4m3, seed=3, new=new)
+    case.table[1, 1], case.table[1, 3] = case.n_pages, -1
+    attend(case, 4, weight=PROMPT if new else WEIGHT)
+    with pytest.raises(hip.LadderHipError, match="page"):
+        hip.raise_on_device_error(DEV)
+    case.table[0, :] = 1 << 30       # none of a sequence's: zeros
+    *_, got = attend(case, 4, weight=PROMPT if new else WEIGHT)
+    assert (got[0] == 0).all()
+    with pytest.raises(hip.LadderHipError, match="page"):
+        hip.raise_on_device_error(DEV)
+    # a length beyond the table's pages: as many keys as these hold
+    case = Case([64, 64], 2, 64, 16, e4m3, seed=3, new=new)
+    case.table = case.table[:, :4].contiguous()
+    full = case.on(DEV, 4)
+    q = rnd(case.rows, 4 * 64).to(DEV)
+    want = full[0].attend(full[1], q, torch.empty_like(q)).clone()
+    if new is None:
+        full[1].lengths[1] = 65
+        assert torch.equal(full[0].attend(full[1], q, torch.empty_like(q)), want)
+        with pytest.raises(hip.LadderHipError, match="position"):
+            hip.raise_on_device_error(DEV)
+        full[1].lengths[1] = -3
+        y = full[0].attend(full[1], q, torch.empty_like(q))
+        assert torch.equal(y[0], want[0]) and (y[1] == 0).all()
+
+
+def test_not_a_number_where_it_is_seen(hip):
+    """NaN in a key or a value of one sequence is that sequence's alone; an infinite value goes through."""
+    for new in (None, [3, 4]):
+        case = Case([40, 50], 1, 64, 16, False, seed=4, new=new)
+        page = int(case.table[0, 0])
+        case.v[page, 0, 2, 5] = math.nan
+        case.v[page, 0, 3, 6] = math.inf
+        cache, batch = case.on(DEV, 2)
+        q = rnd(case.rows, 128).to(DEV)
+        y = cache.attend(batch, q, torch.empty_like(q)).view(case.rows, 2, 64)
+        first = 1 if new is None else 3
+        assert y[:first, :, 5].isnan().all() and (y[:first, :, 6] == math.inf).all()
+        assert y[:first, :, :5].isfinite().all() and y[first:].isfinite().all()
+        case.k[page, 0, 1, 0] = math.nan
+        cache, batch = case.on(DEV, 2)
+        y = cache.attend(batch, q, torch.empty_like(q))
+        assert y[:first].isnan().all() and y[first:].isfinite().all()
+
+
+def test_offsets_beyond_32_bits(hip):
+    """Pages whose bytes and whose elements lie beyond 2^32."""
+    hq, hkv, hd, page = 8, 8, 128, 256
+    n_pages = (1 << 32) // (hkv * page * hd) + 3
+    from gpt_fast.utils import PagedKVCache
+    for dtype in (BF, E4M3):
+        cache = PagedKVCache(n_pages, page, hkv, hd, dtype, device=DEV)
+        table = torch.tensor([[n_pages - 1, 0, n_pages - 2]], dtype=torch.int32, device=DEV)
+        n = 2 * page + 9
+        i = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)
+        batch = cache.batch(table, i(n), hq, starts=i(0, n), rows=n)
+        qkv = rnd(n, (hq + 2 * hkv) * hd, seed=1).to(DEV)
+        q, k, v, y = (torch.empty(n, hq * hd, dtype=BF, device=DEV) for _ in range(4))
+        cache.write(batch, qkv, q)
+        cache.read(batch, k, v)
+        cache.attend(batch, q, y)
+        one = cache.batch(table, i(n), hq)
+        y1 = cache.attend(one, q[-1:], torch.empty_like(q[-1:]))
+        small = PagedKVCache(3, page, hkv, hd, dtype, device=DEV)
+        t2 = i(1, 2, 0)[None]
+        b2 = small.batch(t2, i(n), hq, starts=i(0, n), rows=n)
+        q2, k2, v2, y2 = (torch.empty_like(q) for _ in range(4))
+        small.write(b2, qkv, q2)
+        small.read(b2, k2, v2)
+        small.attend(b2, q2, y2)
+        for a, b in ((q, q2), (k, k2), (v, v2), (y, y2), (y1, small.attend(small.batch(t2, i(n), hq), q2[-1:], torch.empty_like(q2[-1:])))):
+            assert torch.equal(a, b)
+        if dtype == BF:
+            assert torch.equal(k, qkv[:, hq * hd:(hq + hkv) * hd])
+        del cache, batch, one
+        torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------------------------------ together
+
+@pytest.mark.parametrize("dtype", [BF, E4M3])
+def test_prompts_then_tokens_as_a_server_runs_them(hip, dtype):
+    """Three sequences: prompts together in one call, a portion for one of them, then tokens in a captured graph whose table and
+    lengths advance on the device, one sequence leaving and its page going to another; every step against the oracle on what the
+    cache holds, read back."""
+    from gpt_fast.utils import PagedKVCache
+    hq, hkv, hd, page = 4, 2, 64, 16
+    cache = PagedKVCache(24, page, hkv, hd, dtype, device=DEV)
+    g = torch.Generator().manual_seed(1)
+    angle = torch.rand(200, hd // 2, generator=g) * 6.28
+    rope = torch.stack([angle.cos(), angle.sin()], -1).to(BF).to(DEV)
+    table = torch.randperm(24, generator=g).to(torch.int32).view(3, 8)
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    dev_table = table.to(DEV)
+
+    def check(batch, q, y, lengths, starts, weight):
+        whole = cache.batch(dev_table, i(lengths), hq, starts=i([sum(lengths[:b]) for b in range(4)]), rows=max(1, sum(lengths)))
+        k, v = (torch.empty(sum(lengths), hkv * hd, dtype=BF, device=DEV) for _ in range(2))
+        cache.read(whole, k, v)
+        kp, vp = (torch.zeros(24, hkv, page, hd, dtype=F64) for _ in range(2))
+        for r, _, _, p, s in O.places(table, lengths, whole.starts.tolist(), page):
+            kp[p, :, s], vp[p, :, s] = k[r].cpu().double().view(hkv, hd), v[r].cpu().double().view(hkv, hd)
+        want, spread, size = O.attention(q.cpu().view(-1, hq, hd), kp, vp, table, lengths, starts, hd ** -0.5)
+        off = (y.cpu().double().view(want.shape) - want).abs() / bound(want, spread, size, max(lengths), hd, weight)
+        assert off.max() <= 1
+
+    lengths, new = [30, 17, 50], [30, 17, 50]
+    for lengths, new in (([30, 17, 50], [30, 17, 50]), ([30, 37, 50], [0, 20, 0])):
+        starts = [sum(new[:b]) for b in range(4)]
+        batch = cache.batch(dev_table, i(lengths), hq, starts=i(starts), rows=starts[-1])
+        qkv = rnd(starts[-1], (hq + 2 * hkv) * hd, seed=sum(lengths)).to(DEV)
+        q, y = (torch.empty(starts[-1], hq * hd, dtype=BF, device=DEV) for _ in range(2))
+        cache.write(batch, qkv, q, rope)
+        cache.attend(batch, q, y)
+        check(batch, q, y, lengths, starts, PROMPT)
+    step = cache.batch(dev_table, i(lengths), hq)
+    qkv = torch.zeros(3, (hq + 2 * hkv) * hd, dtype=BF, device=DEV)
+    y = torch.empty(3, hq * hd, dtype=BF, device=DEV)
+
+    def once():
+        cache.write(step, qkv, qkv[:, :hq * hd], rope)
+        cache.attend(step, qkv[:, :hq * hd], y)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    k0, v0 = cache.k_pages.clone(), cache.v_pages.clone()
+    with torch.cuda.stream(side):
+        once()
+    torch.cuda.current_stream().wait_stream(side)
+    cache.k_pages.copy_(k0)
+    cache.v_pages.copy_(v0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        once()
+    for n in range(12):
+        fresh = rnd(3, qkv.shape[1], seed=100 + n).to(DEV)
+        lengths = [x + 1 if x else 0 for x in lengths]
+        if n == 5:
+            lengths[0] = 0                        # leaves
+            table[1, 5:7] = table[0, :2]          # its pages are another's
+            dev_table.copy_(table)
+        step.lengths.copy_(i(lengths))
+        qkv.copy_(fresh)
+        graph.replay()
+        check(step, qkv[:, :hq * hd], y, lengths, None, WEIGHT)
+        graph_y = y.clone()
+        qkv.copy_(fresh)
+        once()                                    # eagerly: the same bits
+        assert torch.equal(y, graph_y)
+    hip.raise_on_device_error(DEV)
+
+
+def test_two_batches_on_two_streams(hip):
+    """Each with a scratch of its own, at once, over and over: the bits of each alone."""
+    case = Case([3000, 17, 900], 2, 128, 16, False, seed=2)
+    q = rnd(3, 8 * 128).to(DEV)
+    work = []
+    for _ in range(2):
+        cache, batch = case.on(DEV, 8)
+        work.append((cache, batch, torch.empty_like(q), torch.cuda.Stream()))
+    want = work[0][0].attend(work[0][1], q, torch.empty_like(q)).clone()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for cache, batch, y, stream in work:
+            with torch.cuda.stream(stream):
+                y.zero_()
+                cache.attend(batch, q, y)
+    torch.cuda.synchronize()
+    assert all(torch.equal(w[2], want) for w in work)
+
+
+def test_the_contiguous_caches_numbers(hip):
+    """On one sequence the paged operators do what lr_rope_kv_write, lr_attn_prefill and lr_attn_decode do: the same cached bits, and outputs
+    within the rounding of either."""
+    from gpt_fast.utils import precompute_freqs_cis
+    hq, hkv, hd, page, n = 8, 2, 128, 32, 150
+    case = Case([n], hkv, hd, page, False, new=[n])
+    cache, batch = case.on(DEV, hq)
+    rope = precompute_freqs_cis(256, hd, 500000).to(DEV)
+    qkv = rnd(n, (hq + 2 * hkv) * hd, seed=3).to(DEV)
+    q, y, y0 = (torch.empty(n, hq * hd, dtype=BF, device=DEV) for _ in range(3))
+    cache.write(batch, qkv, q, rope)
+    kc, vc = (torch.zeros(1, hkv, 160, hd, dtype=BF, device=DEV) for _ in range(2))
+    dense = qkv.clone()
+    pos = torch.arange(n, dtype=torch.int32, device=DEV)
+    hip.rope_kv_write(dense, rope, False, pos, kc, vc, 1, n, hq, hkv, hd)
+    k, v = (torch.empty(n, hkv * hd, dtype=BF, device=DEV) for _ in range(2))
+    cache.read(batch, k, v)
+    assert torch.equal(q, dense[:, :hq * hd])
+    assert torch.equal(k.view(n, hkv, hd).transpose(0, 1), kc[0, :, :n]) and torch.equal(v.view(n, hkv, hd).transpose(0, 1), vc[0, :, :n])
+    cache.attend(batch, q, y)
+    hip.attn_prefill(dense, kc, vc, pos, y0, 1, n, hq, hkv, hd)
+    clean = lambda t: torch.nan_to_num(t.cpu().double())
+    want, spread, size = O.attention(q.cpu().view(n, hq, hd), clean(cache.k_pages), clean(cache.v_pages), case.table, [n], [0, n], hd ** -0.5)
+    near = bound(want, spread, size, n, hd, PROMPT)
+    for got in (y, y0):
+        assert ((got.cpu().double().view(want.shape) - want).abs() <= near).all()
+
+
+def test_refusals(hip):
+    case = Case([20, 20], 2, 64, 16, False)
+    cache, batch = case.on(DEV, 4)
+    q = rnd(2, 256).to(DEV)
+    y = torch.empty_like(q)
+    for bad in (q.float(), q[:, :128], q.t().contiguous().t(), q.cpu()):
+        with pytest.raises(ValueError):
+            cache.attend(batch, bad, y)
+        with pytest.raises(ValueError):
+            cache.attend(batch, q, bad)
+    with pytest.raises(ValueError):
+        cache.attend(batch, q[:1], y)
+    with pytest.raises(hip.LadderHipError):
+        cache.attend(batch, q[:1], y[:1])                # one row per sequence
+    with pytest.raises(hip.LadderHipError):
+        cache.attend(batch, q, y, scale=0.0)
+    with pytest.raises(ValueError, match="rows"):
+        cache.attend(batch, q.repeat(2, 1), y.repeat(2, 1))
+    other, _ = Case([20, 20], 1, 64, 16, False).on(DEV, 4)
+    with pytest.raises(ValueError, match="pages"):
+        other.attend(batch, q, y)
+    with pytest.raises(ValueError):
+        cache.write(batch, rnd(2, 8 * 64).to(DEV), q, torch.zeros(8, 32, 2, dtype=torch.float16, device=DEV))
+    with pytest.raises(hip.LadderHipError):
+        cache.write(batch, rnd(2, 8 * 64).to(DEV), q, torch.zeros(8, 12, 2, device=DEV))
+    with pytest.raises(hip.LadderHipError, match="not served"):
+        cache.batch(batch.table, batch.lengths, 5)
+    with pytest.raises(AssertionError):
+        cache.batch(batch.table.long(), batch.lengths, 4)

@@ -1,0 +1,128 @@
+"""The paged key-value cache without a GPU: refusals of the C entry points, the oracle's own definitions, the module's bookkeeping."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from oracle import paged_oracle as O
+
+E_NULL, E_ALIGN, E_SHAPE, E_UNSUPPORTED = -1, -2, -3, -4
+
+
+@pytest.fixture(scope="module")
+def hip():
+    from gpt_fast import _hip
+
+    _hip.load()
+    return _hip
+
+
+def descs(hip, **change):
+    """(cache, batch) that are served, with some fields changed.  The addresses are never followed: nothing is launched."""
+    c = dict(k=4096, v=8192, scales=12288, n_pages=10, page=16, n_kv_head=2, head_dim=128, format=1)
+    b = dict(table=64, ld_table=4, lengths=128, starts=192, err=None, B=3, pages=4)
+    for k, v in change.items():
+        (c if k in c else b)[k] = v
+    return hip._PagedCache(**c), hip._PagedBatch(**b)
+
+
+def calls(hip, cache, batch, rows=5, Hq=8, ld=None, scale=0.1, x=1 << 20, rope=None, rot=128, rope_dtype=0, scratch_bytes=1 << 30):
+    lib, c, b = hip.load(), ctypes.byref(cache), ctypes.byref(batch)
+    hd, hkv = max(cache.head_dim, 1), max(cache.n_kv_head, 1)
+    width = ld or (Hq + 2 * hkv) * hd
+    return (lib.lr_paged_write(c, b, x, width, 1 << 21, Hq * hd, rows, Hq, rope, 64, rot, 1, rope_dtype, None),
+            lib.lr_paged_read(c, b, x, ld or hkv * hd, 1 << 21, ld or hkv * hd, rows, None),
+            lib.lr_paged_attention(c, b, x, ld or Hq * hd, 1 << 21, ld or Hq * hd, rows, Hq, scale, 1 << 22, scratch_bytes, None))
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(k=None), E_NULL), (dict(v=None), E_NULL), (dict(scales=None), E_NULL), (dict(table=None), E_NULL), (dict(lengths=None), E_NULL),
+    (dict(k=4100), E_ALIGN), (dict(v=4104), E_ALIGN), (dict(scales=12290), E_ALIGN), (dict(table=66), E_ALIGN), (dict(lengths=129), E_ALIGN),
+    (dict(starts=193), E_ALIGN), (dict(err=6), E_ALIGN),
+    (dict(n_pages=0), E_SHAPE), (dict(n_kv_head=0), E_SHAPE), (dict(page=0), E_SHAPE), (dict(head_dim=-64), E_SHAPE), (dict(B=0), E_SHAPE),
+    (dict(pages=0), E_SHAPE), (dict(ld_table=3), E_SHAPE), (dict(n_kv_head=3), E_SHAPE),
+    (dict(page=8), E_UNSUPPORTED), (dict(page=24), E_UNSUPPORTED), (dict(page=512), E_UNSUPPORTED), (dict(head_dim=96), E_UNSUPPORTED),
+    (dict(head_dim=256), E_UNSUPPORTED), (dict(format=2), E_UNSUPPORTED), (dict(B=65536), E_UNSUPPORTED),
+    (dict(page=256, pages=(1 << 22) + 1, ld_table=1 << 23), E_UNSUPPORTED),
+    (dict(starts=None), E_SHAPE),      # one row per sequence: 3, not 5
+])
+def test_descriptors_are_checked_by_every_entry_point(hip, change, code):
+    got = calls(hip, *descs(hip, **change))
+    if change == dict(n_kv_head=3):    # 8 q heads on 3: a read has no q heads
+        got = got[0], got[2]
+    assert set(got) == {code}
+    cache, batch = descs(hip, **change)
+    if change not in (dict(starts=None),):
+        assert hip.load().lr_paged_attention_scratch_bytes(ctypes.byref(cache), ctypes.byref(batch), 5, 8) == 0
+
+
+def test_arguments_are_checked(hip):
+    d = descs(hip)
+    lib = hip.load()
+    for n in (None,):
+        assert lib.lr_paged_write(n, ctypes.byref(d[1]), 16, 8, 16, 8, 1, 8, None, 0, 0, 0, 0, None) == E_NULL
+        assert lib.lr_paged_read(ctypes.byref(d[0]), n, 16, 8, 16, 8, 1, None) == E_NULL
+        assert lib.lr_paged_attention(n, n, 16, 8, 16, 8, 1, 8, 1.0, 16, 1 << 30, None) == E_NULL
+    assert set(calls(hip, *d, rows=0)) == {E_SHAPE}
+    assert set(calls(hip, *d, x=None)) == {E_NULL}
+    assert set(calls(hip, *d, x=(1 << 20) + 8)) == {E_ALIGN}
+    assert calls(hip, *d, ld=255)[1] == E_SHAPE and set(calls(hip, *d, ld=12 * 128 + 4)) == {E_ALIGN}
+    assert calls(hip, *d, ld=8)[::2] == (E_SHAPE, E_SHAPE)
+    assert calls(hip, *d, Hq=7)[::2] == (E_SHAPE, E_SHAPE)
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        assert calls(hip, *d, scale=scale)[2] == E_SHAPE
+    assert calls(hip, *d, scratch_bytes=0)[2] == E_SHAPE
+    assert calls(hip, *d, rope=64, rot=144)[0] == E_SHAPE and calls(hip, *d, rope=64, rot=0)[0] == E_SHAPE
+    assert calls(hip, *d, rope=64, rot=24)[0] == E_UNSUPPORTED and calls(hip, *d, rope=64, rope_dtype=2)[0] == E_UNSUPPORTED
+    assert calls(hip, *d, rope=68)[0] == E_ALIGN
+
+
+def test_scratch_grows_with_what_is_served(hip):
+    lib = hip.load()
+    size = lambda rows, Hq, **c: (lambda d: lib.lr_paged_attention_scratch_bytes(ctypes.byref(d[0]), ctypes.byref(d[1]), rows, Hq))(descs(hip, **c))
+    assert size(5, 8) > 0
+    assert size(0, 8) == 0 and size(5, 7) == 0
+    for kw in (dict(), dict(starts=None)):
+        for a, b in (((1, 8), (64, 8)), ((64, 8), (500, 8)), ((8, 8), (8, 16))):
+            assert size(*a, **kw) <= size(*b, **kw)
+
+
+def test_module_bookkeeping():
+    from gpt_fast.utils import PagedKVCache
+
+    c = PagedKVCache(5, 32, 2, 64)
+    assert c.scales is None and c.shape == (2, 32, 64) and c.k_pages.dtype == torch.bfloat16
+    c = PagedKVCache(5, 32, 2, 64, torch.float8_e4m3fn)
+    assert tuple(c.scales.shape) == (5, 2, 2, 32) and c.scales.dtype == torch.uint8
+    c.to(torch.float32)          # a model's type is not its cache's
+    assert c.k_pages.dtype == torch.float8_e4m3fn and c.scales.dtype == torch.uint8
+    assert set(c.state_dict()) == {"k_pages", "v_pages", "scales"}
+    with pytest.raises(AssertionError):
+        PagedKVCache(5, 32, 2, 64, torch.float32)
+    t = torch.zeros(2, 3, dtype=torch.int32)
+    with pytest.raises(AssertionError, match="rows"):
+        c.batch(t, t[:, 0], 4, starts=torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(AssertionError):      # device tensors only
+        c.batch(t, torch.zeros(2, dtype=torch.int32), 4)
+
+
+def test_the_oracle_quantises_as_defined():
+    x = torch.tensor([[448.0, -1.0], [449.0, 1.0], [0.0, 0.0], [448 * 2.0 ** -20, 1e-9], [math.inf, 3.0], [1e-40, 0.0], [-896.0, 0.875]])
+    q, byte = O.quantise(x)
+    assert byte.tolist() == [127, 128, 1, 107, 120, 1, 128]
+    v = O.values(q[:, None, None], torch.stack([byte, byte], 1)[:, None, :, None])[:, 0, 0]
+    assert v[0].tolist() == [448, -1] and v[1].tolist() == [448, 1] and v[2].tolist() == [0, 0] and v[6].tolist() == [-896, 0.875]
+    assert math.isnan(v[4, 0]) and v[4, 1] == 3
+    y = torch.randn(400, 64, generator=torch.Generator().manual_seed(1))
+    q, byte = O.quantise(y)
+    back = O.values(q[:, None, None], torch.stack([byte, byte], 1)[:, None, :, None])[:, 0, 0]
+    step = torch.exp2(byte.double() - 127)[:, None]
+    assert ((back - y.double()).abs() <= torch.maximum(2.0 ** -4 * y.double().abs(), 2.0 ** -10 * step)).all()
+    assert torch.equal(back.to(torch.bfloat16).double(), back)     # exact in bf16
+
+
+def test_the_oracle_places_rows():
+    table = torch.tensor([[4, 2, 9], [1, 0, 3]])
+    assert O.places(table, [17, 0], None, 16) == [(0, 0, 16, 2, 0)]
+    assert O.places(table, [17, 3], [0, 2, 5], 16) == [(0, 0, 15, 4, 15), (1, 0, 16, 2, 0), (2, 1, 0, 1, 0), (3, 1, 1, 1, 1), (4, 1, 2, 1, 2)]
