@@ -42,7 +42,7 @@ FLAGS = [
 
 # per-source additions: the prefill attention rescales its matrix-core accumulators with vector instructions; kept
 # in ordinary vector registers (not the accumulation registers) that costs no copies
-PER_SOURCE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+PER_SOURCE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"], "paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _stale(target, deps):

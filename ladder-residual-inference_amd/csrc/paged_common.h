@@ -68,7 +68,9 @@ static inline int paged_arguments(const lr_paged_cache_t* cache, const lr_paged_
   if (cache->format == LR_CACHE_E4M3) LR_REQUIRE_PTR(cache->scales);
   if (cache->head_dim != 64 && cache->head_dim != 128) return LR_E_UNSUPPORTED;
   if (cache->page < 16 || cache->page > 256 || (cache->page & (cache->page - 1))) return LR_E_UNSUPPORTED;
-  if (batch->B > 65535 || (int64_t)batch->pages * cache->page > (1 << 30)) return LR_E_UNSUPPORTED;   // (positions and tiles are 32-bit numbers)
+  // (positions, and tiles of 32 keys of all sequences, are 32-bit numbers)
+  const int64_t most = (int64_t)batch->pages * cache->page;
+  if (batch->B > 65535 || most > (1 << 30) || batch->B * (most / 32 + 1) >= 0x7fffffff) return LR_E_UNSUPPORTED;
   c.k = (u8*)cache->k;
   c.v = (u8*)cache->v;
   c.scales = (u8*)cache->scales;
