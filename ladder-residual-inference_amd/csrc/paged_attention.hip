@@ -2,6 +2,7 @@
 #include "paged_common.h"
 
 #include <atomic>
+#include <type_traits>
 
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 
@@ -546,76 +547,479 @@ static int launch_paged_decode(const PagedCache& c, const PagedBatch& t, const P
   return lr_launch_status();
 }
 
-// ------------------------------------------------------------------------------------ prompts
-// One wave per (row, q head): 64 keys at a time, a lane one key's score, then 64 values weighted, a lane HD / 64 dimensions.
-template <int HD, bool E4M3>
-__global__ __launch_bounds__(64) void k_paged_attention(const PagedCache c, const PagedBatch t, const PagedQuery a) {
-  constexpr int ROW = HD * (E4M3 ? 1 : 2), D = HD / 64;
-  const int row = blockIdx.x, h = blockIdx.y, kvh = h / (a.Hq / c.Hkv), lane = threadIdx.x;
-  int b = row, back = 1;
-  if (t.starts) {
-    b = paged_sequence(t, row);
-    if (b >= t.B) return;
-    back = t.starts[b + 1] - row;
+// ------------------------------------------------------------------------------------ rows of prompts
+// A kv head's rows of a sequence are its tokens' q heads, token after token: row r is token r / G, head r % G.  A workgroup has 128 of them,
+// a wave 32, whatever G is: the columns of the products
+//   S^T[key][row] = K q^T,   O^T[dim][row] += V^T P^T
+// on the matrix cores (32x32x16).  A column is a lane, so maxima, sums and factors are a lane's own, and the 16 scores that it holds of 32 keys are, in
+// their order, the second product's operand.  Weights enter as bf16 and so they do the sum that divides them: y is off by the weights'
+// rounding, 2^-9 of each at random, about as much as y's own rounding (1.41 times the error of y rounded from exact sums, where keys
+// are many).  Keys come 64 at a time into one of two buffers, one barrier per 64; bf16 by loads straight into LDS, e4m3 through registers, expanded on
+// the way with its row's power of two: from there on the two are the same.
+// Few rows: a workgroup's keys are cut among several, whose results a second launch puts together.
+constexpr int PROMPT_ROWS = 128, PROMPT_KEYS = 64;
+constexpr int PROMPT_SPLIT_KEYS = 256;   // a part of a row's keys has at least so many
+
+struct PagedPrompt {
+  const u16* q;
+  int64_t ldq;
+  u16* y;
+  int64_t ldy;
+  int rows, Hq, n_split, bound;   // bound: blocks of a kv head at most
+  float scale;
+  float *o_part, *ml_part;        // [block][part][128][HD], [..][128][2]
+};
+
+// Which rows a block has.
+struct PromptBlock {
+  int b, row0, n, length, r0;     // sequence, its first row of the call and their number, its keys; the block's first row of the kv head's
+};
+// Blocks of a kv head, last ones first (they see the most keys).  false: there are fewer.
+__device__ __forceinline__ bool prompt_block(const PagedCache& c, const PagedBatch& t, int rows, int G, int index, PromptBlock& at) {
+  const int lane = threadIdx.x & 63;
+  int start = 0, n = 0, blocks = 0, upto = 0, total = 0;
+  auto look = [&](int from) {
+    const int i = from + lane;
+    start = i < t.B ? t.starts[i] : 0;
+    n = i < t.B ? t.starts[i + 1] - start : 0;
+    n = start < 0 || start > rows || n < 0 ? 0 : min(n, rows - start);
+    blocks = (int)(((int64_t)n * G + PROMPT_ROWS - 1) / PROMPT_ROWS);
+    upto = blocks;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(upto, o, 64);
+      upto += lane >= o ? u : 0;
+    }
+    return __builtin_amdgcn_readlane(upto, 63);
+  };
+  for (int i = 0; i < t.B; i += 64) total += look(i);
+  if (index >= total) return false;
+  index = total - 1 - index;
+  int b0 = 0, before = 0;
+  if (t.B > 64)
+    for (;; b0 += 64) {
+      const int k = look(b0);
+      if (index < before + k || b0 + 64 >= t.B) break;
+      before += k;
+    }
+  int s = __popcll(__ballot(before + upto <= index));
+  s = s > 63 ? 63 : s;
+  at.b = b0 + s;
+  at.row0 = __builtin_amdgcn_readlane(start, s);
+  at.n = __builtin_amdgcn_readlane(n, s);
+  at.r0 = (index - before - __builtin_amdgcn_readlane(upto - blocks, s)) * PROMPT_ROWS;
+  at.length = __builtin_amdgcn_readfirstlane(paged_length(t, c.shift, at.b));
+  return true;
+}
+// keys that the block's last row sees
+__device__ __forceinline__ int prompt_keys(const PromptBlock& at, int G) {
+  const int last = min(at.r0 + PROMPT_ROWS, at.n * G) - 1;
+  return max(0, at.length - at.n + last / G + 1);
+}
+// and into how many parts they are cut
+__device__ __forceinline__ int prompt_parts(int keys, int n_split) { return max(1, min(n_split, (keys + PROMPT_SPLIT_KEYS - 1) / PROMPT_SPLIT_KEYS)); }
+
+template <int HD, int KSP>
+struct PromptLds {
+  static constexpr int ROW = HD * 2, TILE = PROMPT_KEYS * ROW, STAGE = 2 * TILE;   // a portion's keys or values; both
+  static constexpr int MERGE = KSP == 2 ? 4 * (HD / 2 + 2) * 64 * 4 : 0;
+  static constexpr int BYTES = 2 * STAGE > MERGE ? 2 * STAGE : MERGE;
+};
+// the place among a row's 16-byte pieces is the piece's number XOR this: 16 lanes reading one piece of 16 consecutive keys, and 16 reading
+// four neighbouring pieces of four keys, touch every bank once
+template <int HD>
+__device__ __forceinline__ int prompt_k_place(int key) { return HD == 128 ? key & 15 : (key >> 1) & 7; }
+template <int HD>
+__device__ __forceinline__ int prompt_v_place(int key) { return HD == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2; }
+
+// KSP 2: eight waves, the second four the second 32 keys of every portion for the same rows; their results meet in LDS.
+template <int HD, bool E4M3, int KSP, bool SPLIT>
+__global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache c, const PagedBatch t, const PagedPrompt a) {
+  using L = PromptLds<HD, KSP>;
+  constexpr int KS = HD / 16, DT = HD / 32;   // k-steps of the score product; 32-row tiles of O^T
+  constexpr int NW = 4 * KSP, RB = L::ROW, PIECES = RB / 16;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char prompt_lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = KSP == 2 ? wave >> 2 : 0, w4 = wave & 3, col = lane & 31, half = lane >> 5;
+  const int G = a.Hq / c.Hkv;
+  // (workgroup i runs on XCD i % 8: the blocks of a kv head meet in few L2s)
+  const int kvh = blockIdx.x % c.Hkv, item = blockIdx.x / c.Hkv, split = SPLIT ? item % a.n_split : 0, index = SPLIT ? item / a.n_split : item;
+  PromptBlock at;
+  if (!prompt_block(c, t, a.rows, G, index, at)) return;
+  const int nkeys = prompt_keys(at, G), portions = (nkeys + PROMPT_KEYS - 1) / PROMPT_KEYS;
+  int t_first = 0, t_end = nkeys;
+  if constexpr (SPLIT) {
+    const int parts = prompt_parts(nkeys, a.n_split);
+    if (split >= parts) return;
+    t_first = (int)((int64_t)portions * split / parts) * PROMPT_KEYS;
+    t_end = min(nkeys, (int)((int64_t)portions * (split + 1) / parts) * PROMPT_KEYS);
   }
-  const int seen = paged_length(t, c.shift, b) - back + 1;   // keys
-  const u16* const q = a.q + row * a.ldq + h * HD;
-  float m = -INFINITY, l = 0.0f, o[D] = {};
-  for (int k0 = 0; k0 < seen; k0 += 64) {
-    const int key = k0 + lane;
-    int page = -1;
-    if (key < seen) {
-      page = t.table[b * t.ld_table + (key >> c.shift)];
-      if (page < 0 || page >= c.n_pages) {
-        page = -1;
+  // this lane's row, the last key that it sees, and the smallest and largest of the wave's
+  const int n_rows = at.n * G, r = at.r0 + w4 * 32 + col, token = r / G, ahead = at.length - at.n;
+  const bool valid = r < n_rows;
+  const int p = valid ? ahead + token : -1;
+  const int wr0 = at.r0 + w4 * 32;
+  const int pmin = __builtin_amdgcn_readfirstlane(ahead + wr0 / G), pmax = __builtin_amdgcn_readfirstlane(wr0 < n_rows ? ahead + (min(wr0 + 32, n_rows) - 1) / G : -1);
+  const int64_t my_row = at.row0 + (valid ? token : 0);
+  const int head = kvh * G + (valid ? r - token * G : 0);
+
+  // the pages of 16 keys each, 64 of these at a time; which are not there
+  const int32_t* const row = t.table + (int64_t)at.b * t.ld_table;
+  int pages, groups0;
+  unsigned long long gone;
+  auto pages_from = [&](int key0) {
+    groups0 = key0;
+    const int key = key0 + 16 * lane;
+    pages = -1;
+    bool bad = false;
+    if (key < t_end) {
+      pages = row[key >> c.shift];
+      bad = (u32)pages >= (u32)c.n_pages;
+      if (bad) {
+        pages = -1;
         if (t.err) *t.err = LR_DEV_PAGE_RANGE;
       }
     }
-    const int slot = key & ((1 << c.shift) - 1);
-    float s = -INFINITY, vs = 1.0f;
-    if (page >= 0) {
-      const u8* const k = c.k + paged_offset<ROW>(c, page, kvh) + slot * ROW;
-      float sum = 0.0f;
-      for (int d = 0; d < HD; ++d) {
-        float x;
-        if constexpr (E4M3) x = __builtin_amdgcn_cvt_f32_fp8(k[d], 0);
-        else x = bf_to_f(reinterpret_cast<const u16*>(k)[d]);
-        sum = fmaf(x, bf_to_f(q[d]), sum);
-      }
-      s = sum * a.scale;
-      if constexpr (E4M3) {
-        const u8* const e = c.scales + paged_scales(c, page, kvh) + slot;
-        s *= paged_scale(e[0]);
-        vs = paged_scale(e[1 << c.shift]);
+    gone = __ballot(bad);
+  };
+  pages_from(t_first);
+
+  // q as the products' second operand: k-step i holds elements 16 i + 8 half .. + 8 of this lane's row
+  u32x4_t qb[KS];
+  {
+    const u16* const qrow = a.q + my_row * a.ldq + head * HD;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      const uint4 x = ld16(qrow + 16 * i + 8 * half);
+      qb[i] = u32x4_t{x.x, x.y, x.z, x.w};
+    }
+#pragma unroll
+    for (int i = 0; i < KS; ++i) asm volatile("" : "+v"(qb[i]));   // (waited for here, not behind the loads below)
+  }
+  f32x16_t o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
+  float m = -INFINITY, l = 0.0f;   // m: reference point in raw scores; l: this lane's half of the row's sum
+  const float c2 = a.scale * 1.4426950408889634f, tau = PAGED_TAU2 / c2;
+
+  // ---- loads of a portion
+  constexpr int RPL = 1024 / RB, LOADS = PROMPT_KEYS / RPL / NW;   // bf16: rows per load instruction; a wave's loads of K or V
+  const u32 lds0 = __builtin_amdgcn_readfirstlane((u32)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)prompt_lds);
+  const int lrow = lane / PIECES, place = lane % PIECES;
+  static_assert(NW * RPL % 16 == 0 && RPL % 4 == 0, "a lane's piece is the same for all of a wave's loads");
+  const int kvoff = lrow * RB + (place ^ prompt_k_place<HD>(wave * RPL + lrow)) * 16;
+  const int vvoff = lrow * RB + (place ^ prompt_v_place<HD>(lrow)) * 16;
+  auto stage = [&](int t0, int buf) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int first = (i * NW + wave) * RPL;
+      const int page = __builtin_amdgcn_readlane(pages, (t0 - groups0 + first) >> 4);
+      const int64_t off = paged_offset<RB>(c, page < 0 ? 0 : page, kvh);
+      const bool ok = page >= 0 && t0 + first + lrow < t_end;
+      const int soff = ((t0 + first) & ((1 << c.shift) - 1)) * RB;
+      const u32 to = lds0 + buf * L::STAGE + (i * NW + wave) * 1024;
+      paged_load16(paged_resource(c.k + off), ok ? kvoff : PAGED_OUT, soff, to);
+      paged_load16(paged_resource(c.v + off), ok ? vvoff : PAGED_OUT, soff, to + L::TILE);
+    }
+  };
+  // e4m3: 16 elements of K's or V's rows per piece
+  constexpr int NP = 8 * HD / (256 * KSP), HP = HD / 16;
+  uint4 raw[E4M3 ? NP : 1];
+  u32 byte[E4M3 ? NP : 1];
+  auto fetch = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int x = i * 256 * KSP + tid, value = x >= 4 * HD, key = x % (4 * HD) / HP, pc = x % HP;
+      const int page = __shfl(pages, (t0 - groups0 + key) >> 4, 64);
+      const bool ok = page >= 0 && t0 + key < t_end;
+      const int slot = (t0 + key) & ((1 << c.shift) - 1), safe = ok ? page : 0;
+      raw[i] = ld16((value ? c.v : c.k) + paged_offset<HD>(c, safe, kvh) + slot * HD + pc * 16);
+      byte[i] = c.scales[paged_scales(c, safe, kvh) + (value << c.shift) + slot];
+      if (!ok) raw[i] = make_uint4(0, 0, 0, 0), byte[i] = 127;
+    }
+  };
+  auto expand = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int x = i * 256 * KSP + tid, value = x >= 4 * HD, key = x % (4 * HD) / HP, pc = x % HP;
+      const float s = paged_scale(byte[i]);
+      auto two = [&](u32 lo, u32 hi) {
+        return make_uint4(__builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false)),
+                          __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true)),
+                          __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false)),
+                          __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true)));
+      };
+      unsigned char* const to = prompt_lds + buf * L::STAGE + value * L::TILE + key * RB;
+      const int swap = value ? prompt_v_place<HD>(key) : prompt_k_place<HD>(key);
+      *reinterpret_cast<uint4*>(to + ((2 * pc) ^ swap) * 16) = two(raw[i].x, raw[i].y);
+      *reinterpret_cast<uint4*>(to + ((2 * pc + 1) ^ swap) * 16) = two(raw[i].z, raw[i].w);
+    }
+  };
+
+  // where this lane reads: the K fragments of key `col` of a tile (k-step i: XOR 32 i), and 4 dimensions of key (lane % 16) / 4 of the
+  // four keys whose values 16 lanes exchange (32-row tile d of O^T)
+  const int kat = (part * 32 + col) * RB + ((half ^ prompt_k_place<HD>(col)) * 16);
+  const int vkey = (lane & 15) >> 2;
+  int vat[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) {
+    const int piece = 4 * d + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+    vat[d] = L::TILE + (part * 32 + 4 * half + vkey) * RB + (piece ^ prompt_v_place<HD>(vkey)) * 16 + (lane & 1) * 8;
+  }
+  // N tiles of 32 keys of the portion at t0
+  auto tiles = [&](auto N_, int t0, int buf) {
+    constexpr int N = decltype(N_)::value;
+    const int tk = t0 + part * 32;
+    const unsigned char* const from = prompt_lds + buf * L::STAGE;
+    f32x16_t sacc[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) sacc[n][v] = 0.0f;
+    u32x4_t ka[KS][N];
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int n = 0; n < N; ++n) ka[i][n] = *reinterpret_cast<const u32x4_t*>(from + (kat ^ (32 * i)) + n * 32 * RB);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        sacc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, ka[i][n]), __builtin_bit_cast(bf16x8_t, qb[i]), sacc[n], 0, 0, 0);
+    // element v of tile n: key tk + 32 n + (v / 4) * 8 + half * 4 + v % 4
+    const u32 lost = (u32)(gone >> ((tk - groups0) >> 4)) & (N == 2 ? 15 : 3);
+    if (tk + 32 * N - 1 > pmin || lost) {   // uniform
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int key = tk + 32 * n + (v / 4) * 8 + half * 4 + (v % 4);
+          sacc[n][v] = key <= p && !(lost >> (2 * n + v / 8) & 1) ? sacc[n][v] : -INFINITY;
+        }
+    }
+    float top = sacc[0][0];
+#pragma unroll
+    for (int v = 1; v < 16 * N; ++v) top = __builtin_amdgcn_fmed3f(top, sacc[v / 16][v % 16], INFINITY);   // (the larger; see k_attn_prefill_mfma)
+    {
+      const u32 u = __float_as_uint(top);
+      const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+      top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+    }
+    const bool grow = top > m + tau;   // m = -inf: any finite maximum
+    const float mn = grow ? top : m, nmc = mn == -INFINITY ? 0.0f : -mn * c2;
+    if (__any(grow)) {
+      const float corr = grow ? exp2_hw((m - mn) * c2) : 1.0f;   // m = -inf: 0
+      l *= corr;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] *= corr;
+    }
+    m = mn;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      u32x4_t pw[2];
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u32 w = pack_bf2(exp2_hw(fmaf(sacc[n][8 * h2 + 2 * j], c2, nmc)), exp2_hw(fmaf(sacc[n][8 * h2 + 2 * j + 1], c2, nmc)));   // masked: 0
+          l += bf_lo(w) + bf_hi(w);
+          pw[h2][j] = w;
+        }
+      // k-step h2 covers keys 16 h2 + {0..3, 8..11} + 4 half of the tile, in the order of sacc
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2) {
+        bf16x8_t va[DT];
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const unsigned char* const v0 = from + vat[d] + (n * 32 + 16 * h2) * RB;
+          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)(v0));
+          const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)(v0 + 8 * RB));
+          va[d] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[d], __builtin_bit_cast(bf16x8_t, pw[h2]), o[d], 0, 0, 0);
       }
     }
-    const float mn = fmaxf(m, wave_max(s));
-    if (mn == -INFINITY) continue;
-    const float corr = expf(m - mn), p = expf(s - mn);
-    m = mn;
-    l = l * corr + wave_sum(p);
-#pragma unroll
-    for (int i = 0; i < D; ++i) o[i] *= corr;
-    for (int j = 0; j < 64; ++j) {
-      const int pj = __builtin_amdgcn_readlane(page, j);
-      if (pj < 0) continue;
-      const float w = lr_lane(p, j) * lr_lane(vs, j);
-      const u8* const v = c.v + paged_offset<ROW>(c, pj, kvh) + ((k0 + j) & ((1 << c.shift) - 1)) * ROW;
-#pragma unroll
-      for (int i = 0; i < D; ++i) {
-        float x;
-        if constexpr (E4M3) x = __builtin_amdgcn_cvt_f32_fp8(v[i * 64 + lane], 0);
-        else x = bf_to_f(reinterpret_cast<const u16*>(v)[i * 64 + lane]);
-        o[i] = fmaf(w, x, o[i]);
-      }
+  };
+
+  int buf = 0;
+  if (t_first < t_end) {
+    if constexpr (E4M3) {
+      fetch(t_first);
+      expand(0);
+    } else {
+      stage(t_first, 0);
     }
   }
+  for (int t0 = t_first; t0 < t_end; t0 += PROMPT_KEYS, buf ^= 1) {
+    // the portion has arrived, for all waves, and nobody reads the one before any more
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const bool more = t0 + PROMPT_KEYS < t_end;
+    const unsigned long long gone_now = gone;
+    const int groups_now = groups0;
+    if (more) {
+      if (t0 + PROMPT_KEYS - groups0 == 1024) pages_from(t0 + PROMPT_KEYS);
+      if constexpr (E4M3) fetch(t0 + PROMPT_KEYS);
+      else stage(t0 + PROMPT_KEYS, buf ^ 1);
+    }
+    {
+      const unsigned long long gone_next = gone;
+      const int groups_next = groups0;
+      gone = gone_now;
+      groups0 = groups_now;
+      const int tk = t0 + part * 32;
+      if constexpr (KSP == 2) {
+        if (tk <= pmax) tiles(std::integral_constant<int, 1>{}, t0, buf);
+      } else {
+        if (tk + 32 <= pmax) tiles(std::integral_constant<int, 2>{}, t0, buf);
+        else if (tk <= pmax) tiles(std::integral_constant<int, 1>{}, t0, buf);
+      }
+      gone = gone_next;
+      groups0 = groups_next;
+    }
+    if constexpr (E4M3)
+      if (more) expand(buf ^ 1);
+  }
+  if constexpr (KSP == 2) {
+    // the second four waves' results to the first four
+    __syncthreads();
+    float* const mine = reinterpret_cast<float*>(prompt_lds) + w4 * (HD / 2 + 2) * 64 + lane;
+    if (part) {
 #pragma unroll
-  for (int i = 0; i < D; ++i) a.y[row * a.ldy + h * HD + i * 64 + lane] = f_to_bf(l != 0.0f ? o[i] / l : 0.0f);
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mine[(d * 16 + v) * 64] = o[d][v];
+      mine[(HD / 2) * 64] = m;
+      mine[(HD / 2 + 1) * 64] = l;
+    }
+    __syncthreads();
+    if (part) return;
+    // (-inf, 0, 0: no key seen; -inf, NaN, NaN: only NaN)
+    const float m1 = mine[(HD / 2) * 64], mn = fmaxf(m, m1), ref = mn == -INFINITY ? 0.0f : mn;
+    const float f0 = exp2_hw((m - ref) * c2), f1 = exp2_hw((m1 - ref) * c2);
+    l = l * f0 + mine[(HD / 2 + 1) * 64] * f1;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) o[d][v] = fmaf(o[d][v], f0, mine[(d * 16 + v) * 64] * f1);
+    m = mn;
+  }
+  l += __shfl_xor(l, 32, LR_WAVE);
+  if (!valid) return;
+  // element v of tile d: dimension d * 32 + (v / 4) * 8 + half * 4 + v % 4
+  if (!SPLIT || prompt_parts(nkeys, a.n_split) == 1) {
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    u16* const yrow = a.y + my_row * a.ldy + head * HD;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4) {
+        uint2 w2;
+        w2.x = pack_bf2(o[d][4 * g4] * inv, o[d][4 * g4 + 1] * inv);
+        w2.y = pack_bf2(o[d][4 * g4 + 2] * inv, o[d][4 * g4 + 3] * inv);
+        *reinterpret_cast<uint2*>(yrow + d * 32 + g4 * 8 + half * 4) = w2;
+      }
+  } else {
+    const int64_t place_ = ((int64_t)(kvh * a.bound + index) * a.n_split + split) * PROMPT_ROWS + w4 * 32 + col;
+    float* const to = a.o_part + place_ * HD;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4)
+        *reinterpret_cast<f32x4_t*>(to + d * 32 + g4 * 8 + half * 4) = f32x4_t{o[d][4 * g4], o[d][4 * g4 + 1], o[d][4 * g4 + 2], o[d][4 * g4 + 3]};
+    if (half == 0) *reinterpret_cast<f32x2_t*>(a.ml_part + place_ * 2) = f32x2_t{m * c2, l};
+  }
+}
+
+// The parts of a block's rows together: a workgroup has 16 of its 128 rows.
+template <int HD>
+__global__ __launch_bounds__(256) void k_paged_prompt_join(const PagedCache c, const PagedBatch t, const PagedPrompt a) {
+  const int G = a.Hq / c.Hkv, kvh = blockIdx.x % c.Hkv, index = blockIdx.x / c.Hkv;
+  PromptBlock at;
+  if (!prompt_block(c, t, a.rows, G, index, at)) return;
+  const int parts = prompt_parts(prompt_keys(at, G), a.n_split);
+  if (parts == 1) return;
+  for (int i = threadIdx.x; i < 16 * (HD / 4); i += 256) {
+    const int k = blockIdx.y * 16 + i / (HD / 4), d = i % (HD / 4) * 4, r = at.r0 + k;
+    if (r >= at.n * G) break;
+    const int64_t place = (int64_t)(kvh * a.bound + index) * a.n_split * PROMPT_ROWS + k;
+    float M = -INFINITY, L = 0.0f;
+    f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int u = 0; u < parts; u += 8) {
+      f32x4_t ov[8];
+      f32x2_t ml[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int64_t x = place + (int64_t)min(u + j, parts - 1) * PROMPT_ROWS;
+        ov[j] = *reinterpret_cast<const f32x4_t*>(a.o_part + x * HD + d);
+        ml[j] = *reinterpret_cast<const f32x2_t*>(a.ml_part + x * 2);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (u + j < parts) {
+          const float Mn = fmaxf(M, ml[j][0]), ref = Mn == -INFINITY ? 0.0f : Mn;
+          const float f0 = exp2_hw(M - ref), f1 = exp2_hw(ml[j][0] - ref);
+          L = L * f0 + ml[j][1] * f1;
+          v = v * f0 + ov[j] * f1;
+          M = Mn;
+        }
+    }
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+    u32x2_t out;
+    out.x = pack_bf2(v[0] * inv, v[1] * inv);
+    out.y = pack_bf2(v[2] * inv, v[3] * inv);
+    *reinterpret_cast<u32x2_t*>(a.y + (at.row0 + r / G) * a.ldy + (kvh * G + r % G) * HD + d) = out;
+  }
+}
+
+struct PromptPlan {
+  int bound, n_split;
+  int64_t items;
+  size_t bytes;   // of parts that any number of rows could need
+};
+static PromptPlan prompt_plan(const PagedCache& c, const PagedBatch& t, int hd, int rows, int Hq) {
+  PromptPlan p;
+  const int G = Hq / c.Hkv, cus = lr_num_cus() ? lr_num_cus() : 256;
+  const int64_t some = t.B < rows ? t.B : rows;   // sequences with rows, at most: the last block of each may be short
+  p.items = ((int64_t)rows * G + (PROMPT_ROWS - 1) * some) / PROMPT_ROWS;
+  p.bound = p.items > 0x3fffffff ? 0x3fffffff : (int)p.items;
+  p.items *= c.Hkv;
+  const int64_t most = (((int64_t)t.pages << c.shift) + PROMPT_SPLIT_KEYS - 1) / PROMPT_SPLIT_KEYS;
+  int64_t n = p.items ? cus / p.items : 1;
+  if (n > most) n = most;
+  p.n_split = n < 1 ? 1 : (int)n;
+  p.bytes = most > 1 ? (size_t)cus * PROMPT_ROWS * (hd + 2) * 4 : 0;
+  return p;
+}
+
+template <int HD, bool E4M3, int KSP, bool SPLIT>
+static int launch_prompt_as(const PagedCache& c, const PagedBatch& t, const PagedPrompt& a, unsigned grid, hipStream_t s) {
+  constexpr size_t lds = PromptLds<HD, KSP>::BYTES;
+  static std::atomic<unsigned long long> raised{0};
+  if (!lr_raise_lds_limit(reinterpret_cast<const void*>(&k_paged_prompt<HD, E4M3, KSP, SPLIT>), lds, raised)) return LR_E_LAUNCH;
+  k_paged_prompt<HD, E4M3, KSP, SPLIT><<<dim3(grid), dim3(256 * KSP), lds, s>>>(c, t, a);
+  return lr_launch_status();
+}
+template <int HD, bool E4M3>
+static int launch_prompt(const PagedCache& c, const PagedBatch& t, const PagedQuery& q, void* scratch, hipStream_t s) {
+  const PromptPlan p = prompt_plan(c, t, HD, q.rows, q.Hq);
+  if (p.items * p.n_split > (1 << 24)) return LR_E_UNSUPPORTED;   // (workgroups of a grid)
+  PagedPrompt a = {q.q, q.ldq, q.y, q.ldy, q.rows, q.Hq, p.n_split, p.bound, q.scale, (float*)scratch, nullptr};
+  a.ml_part = a.o_part + (size_t)p.items * p.n_split * PROMPT_ROWS * HD;
+  if (p.n_split == 1) return launch_prompt_as<HD, E4M3, 1, false>(c, t, a, (unsigned)p.items, s);
+  if (const int rc = launch_prompt_as<HD, E4M3, 2, true>(c, t, a, (unsigned)(p.items * p.n_split), s)) return rc;
+  k_paged_prompt_join<HD><<<dim3((unsigned)p.items, PROMPT_ROWS / 16), dim3(256), 0, s>>>(c, t, a);
+  return lr_launch_status();
 }
 
 static size_t paged_scratch(const PagedCache& c, const PagedBatch& t, int hd, bool e4m3, int rows, int Hq) {
-  if (t.starts) return 256;
+  if (t.starts) return 256 + prompt_plan(c, t, hd, rows, Hq).bytes;
   const DecodePlan p = hd == 128 ? (e4m3 ? decode_plan<128, true>(c, t, Hq) : decode_plan<128, false>(c, t, Hq))
                                  : (e4m3 ? decode_plan<64, true>(c, t, Hq) : decode_plan<64, false>(c, t, Hq));
   if (p.groups > 65535) return 0;   // (a grid's second dimension)
@@ -640,6 +1044,7 @@ extern "C" int lr_paged_attention(const lr_paged_cache_t* cache, const lr_paged_
   const int hd = cache->head_dim;
   const bool e4m3 = cache->format == LR_CACHE_E4M3;
   if (rows <= 0 || Hq <= 0 || Hq % c.Hkv || (t.starts == nullptr && rows != t.B)) return LR_E_SHAPE;
+  if ((int64_t)rows * Hq > 0x3fffffff) return LR_E_UNSUPPORTED;
   if (Hq > 65535 || ldq < (int64_t)Hq * hd || ldy < (int64_t)Hq * hd || !(scale > 0.0f && scale < INFINITY)) return LR_E_SHAPE;
   if (ldq % 8 || ldy % 8) return LR_E_ALIGN;
   const size_t need = paged_scratch(c, t, hd, e4m3, rows, Hq);
@@ -650,10 +1055,6 @@ extern "C" int lr_paged_attention(const lr_paged_cache_t* cache, const lr_paged_
   if (t.starts == nullptr)
     return hd == 128 ? (e4m3 ? launch_paged_decode<128, true>(c, t, a, scratch, s) : launch_paged_decode<128, false>(c, t, a, scratch, s))
                      : (e4m3 ? launch_paged_decode<64, true>(c, t, a, scratch, s) : launch_paged_decode<64, false>(c, t, a, scratch, s));
-  const dim3 grid((unsigned)rows, (unsigned)Hq);
-  if (hd == 128 && e4m3) k_paged_attention<128, true><<<grid, dim3(64), 0, s>>>(c, t, a);
-  else if (hd == 128) k_paged_attention<128, false><<<grid, dim3(64), 0, s>>>(c, t, a);
-  else if (e4m3) k_paged_attention<64, true><<<grid, dim3(64), 0, s>>>(c, t, a);
-  else k_paged_attention<64, false><<<grid, dim3(64), 0, s>>>(c, t, a);
-  return lr_launch_status();
+  return hd == 128 ? (e4m3 ? launch_prompt<128, true>(c, t, a, scratch, s) : launch_prompt<128, false>(c, t, a, scratch, s))
+                   : (e4m3 ? launch_prompt<64, true>(c, t, a, scratch, s) : launch_prompt<64, false>(c, t, a, scratch, s));
 }
