@@ -38,8 +38,13 @@ __device__ __forceinline__ i32x4_t paged_resource(const u8* at) {
   return i32x4_t{(int)(u32)(unsigned long long)at, (int)(u32)((unsigned long long)at >> 32) & 0xffff, 0x7fffffff, 0x00020000};
 }
 // 16 (4) bytes per lane from resource + voff + soff to LDS address `lds` + 16 (4) * lane; counted by vmcnt, not by the compiler
+// (ONCE: rows that nobody else reads, non-temporal)
+template <bool ONCE = false>
 __device__ __forceinline__ void paged_load16(const i32x4_t& res, int voff, int soff, u32 lds) {
-  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"{m0}"(lds), "v"(voff), "s"(res), "s"(soff) : "memory");
+  if constexpr (ONCE)
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds" ::"{m0}"(lds), "v"(voff), "s"(res), "s"(soff) : "memory");
+  else
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"{m0}"(lds), "v"(voff), "s"(res), "s"(soff) : "memory");
 }
 __device__ __forceinline__ void paged_load4(const i32x4_t& res, int voff, int soff, u32 lds) {
   asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"{m0}"(lds), "v"(voff), "s"(res), "s"(soff) : "memory");
@@ -75,9 +80,9 @@ struct DecodeTile {
   static constexpr int TILE = 32 * ROW, SCALES = E4M3 ? 512 : 0;       // (256 bytes for the 16-key halves' scales each)
   static constexpr int LDO = HD + 4;                                   // row length of the waves' results when they are put together
   static constexpr int WAVE = 2 * TILE + SCALES;
-  static_assert(16 * LDO * 4 <= WAVE, "");
-  static constexpr int PER_CU = HD == 64 ? 4 : E4M3 ? 3 : 2;            // workgroups that a CU holds, by LDS or registers
-  static constexpr int LDS = 4 * WAVE + 512 + 16;   // (the waves' maxima and sums; a ticket)
+  static constexpr int NW = 4, PER_CU = HD == 64 ? 2 : 1;              // waves of a workgroup; workgroups of a CU
+  static constexpr int RESULT = 16 * LDO * 4;                          // a wave's results
+  static constexpr int LDS = NW * (WAVE + RESULT + 128) + 16;          // (with the waves' maxima and sums, and two tickets)
   // which place among its row's pieces a piece has: its number XOR this.  16 lanes reading a piece of 16 consecutive keys, and 32 lanes
   // reading across the keys that V's products take (0..7 or 8..15 and, e4m3, 16 more), meet no bank of the 64 twice
   static __device__ __forceinline__ int k_place(int row) { return (row * PIECES / 16) & (PIECES - 1); }
@@ -100,16 +105,19 @@ struct PagedDecode {
   u32* tickets;   // [group][B], then [group][block][2]; zero between calls
 };
 
+// What a sequence costs a worker besides its tiles, in tiles (7 us in a row of short sequences for two of them; a tile 0.45 us): as much more room
+// it has on the line.
+constexpr int PAGED_SEQUENCE = 6;
 // A sequence's parts are put together by the last of its workers, of no more than so many at a time: more go through their blocks' last ones.
 constexpr int PAGED_BLOCK = 16;
 
 template <int HD, bool E4M3>
-__global__ __launch_bounds__(256, (DecodeTile<HD, E4M3>::PER_CU)) void k_paged_decode(const PagedCache c, const PagedBatch t, const PagedDecode a) {
+__global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4M3>::PER_CU * DecodeTile<HD, E4M3>::NW / 4)) void k_paged_decode(const PagedCache c, const PagedBatch t, const PagedDecode a) {
   using T = DecodeTile<HD, E4M3>;
-  constexpr int KS = HD / 32, DT = HD / 16;   // k-steps of a score product; 16-dimension tiles of O^T
+  constexpr int KS = HD / 32, DT = HD / 16, NW = T::NW;   // k-steps of a score product; 16-dimension tiles of O^T
   extern __shared__ __attribute__((aligned(1024))) unsigned char paged_lds[];
-  float (*const s_ml)[16][2] = reinterpret_cast<float (*)[16][2]>(paged_lds + 4 * T::WAVE);   // [4]
-  u32* const s_ticket = reinterpret_cast<u32*>(paged_lds + 4 * T::WAVE + 512);
+  float (*const s_ml)[16][2] = reinterpret_cast<float (*)[16][2]>(paged_lds + NW * (T::WAVE + T::RESULT));   // [NW]
+  u32* const s_ticket = reinterpret_cast<u32*>(paged_lds + NW * (T::WAVE + T::RESULT + 128));
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, l4 = lane >> 4;
   const int group = blockIdx.y, kvh = group / a.groups_per_kv, G = a.Hq / c.Hkv;
@@ -117,25 +125,20 @@ __global__ __launch_bounds__(256, (DecodeTile<HD, E4M3>::PER_CU)) void k_paged_d
 
   // ---- which tiles are this worker's
   int b0 = 0;   // lane i looks after sequence b0 + i
-  int len, tiles;
+  int len, tiles, upto;   // its keys, its tiles, and the tiles up to it of the 64 sequences
+  unsigned long long some;   // which of them have tiles
   auto look = [&](int from) {
     b0 = from;
     len = b0 + lane < t.B ? paged_length(t, c.shift, b0 + lane) : 0;
     tiles = (len + 31) >> 5;
+    upto = paged_sums(tiles);
+    some = __ballot(tiles > 0);
   };
-  auto sum_to = [&](int v) {   // inclusive sums over the lanes
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(v, o, 64);
-      v += lane >= o ? u : 0;
-    }
-    return v;
-  };
-  int total = 0, upto = 0;
+  int total = 0, sequences = 0;
   for (int i = 0; i < t.B; i += 64) {
     look(i);
-    upto = sum_to(tiles);
     total += __builtin_amdgcn_readlane(upto, 63);
+    sequences += __popcll(some);
     if (wave == 0) {   // empty places: zeros, one worker each
       unsigned long long empty = __ballot(i + lane < t.B && tiles == 0 && (i + lane) % gridDim.x == blockIdx.x);
       for (; empty; empty &= empty - 1) {
@@ -144,25 +147,32 @@ __global__ __launch_bounds__(256, (DecodeTile<HD, E4M3>::PER_CU)) void k_paged_d
       }
     }
   }
-  const int workers = min((int)gridDim.x, (total + 3) >> 2), w = blockIdx.x;   // (four tiles at least: one for each wave)
+  const int workers = min((int)gridDim.x, max((total + NW - 1) / NW, sequences)), w = blockIdx.x;   // (a tile for each wave, or a sequence)
   if (w >= workers) return;
-  int at = (int)((int64_t)w * total / workers);
-  const int end = (int)((int64_t)(w + 1) * total / workers);
-  // the sequence that tile `at` belongs to: b0 + s, whose first tile is `first`
+  // what a sequence costs besides its tiles, as more room on the line: where workers have one sequence or several; where a sequence has
+  // many workers, it is the same for all of them
+  const int extra = 2 * sequences >= workers ? PAGED_SEQUENCE : 0;
+  total += extra * sequences;
+  auto places_upto = [&]() { return upto + extra * __popcll(some & (~0ull >> (63 - lane))); };   // of the 64 sequences, in all lanes
+  // equal parts, the first `larger` of them a tile more
+  const int each = (u32)total / (u32)workers, larger = total - each * workers;
+  int at = w * each + min(w, larger);
+  const int end = at + each + (w < larger);
+  // the sequence that `at` belongs to: b0 + s, which begins at `first`
   int s, first;
   {
     int before = 0;
     if (t.B > 64) {
       for (int i = 0;; i += 64) {
         look(i);
-        upto = sum_to(tiles);
-        const int n = __builtin_amdgcn_readlane(upto, 63);
-        if (at < before + n) break;
+        const int n = __builtin_amdgcn_readlane(upto, 63) + extra * __popcll(some);
+        if (at < before + n || i + 64 >= t.B) break;
         before += n;
       }
     }
-    s = __popcll(__ballot(before + upto <= at));
-    first = before + __builtin_amdgcn_readlane(upto - tiles, s);
+    const int places = places_upto();
+    s = __popcll(__ballot(before + places <= at)) & 63;
+    first = before + __builtin_amdgcn_readlane(places, s) - __builtin_amdgcn_readlane(tiles, s) - extra;
   }
 
   const u32 lds0 = __builtin_amdgcn_readfirstlane((u32)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)paged_lds) + wave * T::WAVE;
@@ -171,57 +181,129 @@ __global__ __launch_bounds__(256, (DecodeTile<HD, E4M3>::PER_CU)) void k_paged_d
   const float c2 = a.scale * 1.4426950408889634f;   // e^(x scale) = 2^(x c2)
   const float tau = PAGED_TAU2 / c2;
 
-  while (at < end) {
-    const int b = b0 + s, length = __builtin_amdgcn_readlane(len, s), n_tiles = __builtin_amdgcn_readlane(tiles, s);
-    const int from = at - first, to = min(n_tiles, end - first);   // this worker's tiles of the sequence
-    const int32_t* const row = t.table + (int64_t)b * t.ld_table;
-
-    // q as the products' second operand: column = head lane % 16; e4m3: in the order in which K's 16-byte pieces hold the elements
-    bf16x8_t qf[KS];
-    {
-      const u16* const q = a.q + b * a.ldq + (h0 + (l16 < nh ? l16 : 0)) * HD;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        qf[ks] = __builtin_bit_cast(bf16x8_t, ld16(q + (E4M3 ? (ks >> 1) * 64 + l4 * 16 + (ks & 1) * 8 : ks * 32 + l4 * 8)));
+  // this worker's tiles from .. to of the n_tiles of a sequence, the first of which is at `first` of the line, behind the sequence's own cost
+  struct Segment {
+    int b, length, n_tiles, first, from, to;
+  };
+  auto segment = [&]() {
+    Segment g;
+    g.b = b0 + s;
+    g.length = __builtin_amdgcn_readlane(len, s);
+    g.n_tiles = __builtin_amdgcn_readlane(tiles, s);
+    g.first = first + extra;
+    g.from = max(0, at - g.first);
+    g.to = min(g.n_tiles, end - g.first);
+    return g;
+  };
+  // on to the next sequence that has tiles; false: this worker's part of the line ends before its first one
+  auto next_segment = [&](Segment& g) {
+    first += __builtin_amdgcn_readlane(tiles, s) + extra;
+    if (first + extra >= end) return false;
+    unsigned long long others = some & (s == 63 ? 0ull : ~0ull << (s + 1));
+    while (!others) {
+      if (b0 + 64 >= t.B) return false;
+      look(b0 + 64);
+      others = some;
     }
-    // the pages of this wave's next 32 tiles: lane i has that of tile i / 2, its 16-key half i % 2
-    auto pages_of = [&](int tile) {
-      const int key = (tile + 4 * (lane >> 1)) * 32 + (lane & 1) * 16;
-      int p = -1;
-      if (tile + 4 * (lane >> 1) < to && key < length) {
-        p = row[key >> c.shift];
-        if ((u32)p >= (u32)c.n_pages) {
-          p = -1;
-          if (t.err) *t.err = LR_DEV_PAGE_RANGE;
-        }
-      }
-      return p;
-    };
-    int tile = from + wave, j = 0;
-    int pages = pages_of(tile), pages_next = pages_of(tile + 128);
+    s = __builtin_ctzll(others);
+    g = segment();
+    return true;
+  };
+  // q as the products' second operand: column = head lane % 16; e4m3: in the order in which K's 16-byte pieces hold the elements
+  auto load_q = [&](const Segment& g, bf16x8_t* qf) {
+    const u16* const q = a.q + g.b * a.ldq + (h0 + (l16 < nh ? l16 : 0)) * HD;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));   // (waited for here, not behind the loads below)
+    for (int ks = 0; ks < KS; ++ks)
+      qf[ks] = __builtin_bit_cast(bf16x8_t, ld16(q + (E4M3 ? (ks >> 1) * 64 + l4 * 16 + (ks & 1) * 8 : ks * 32 + l4 * 8)));
+  };
+  // the pages of this wave's next 32 tiles from `tile` on: lane i has that of tile i / 2, its 16-key half i % 2
+  auto pages_of = [&](const Segment& g, int tile) {
+    const int key = (tile + NW * (lane >> 1)) * 32 + (lane & 1) * 16;
+    int p = -1;
+    if (tile + NW * (lane >> 1) < g.to && key < g.length) {
+      p = t.table[(int64_t)g.b * t.ld_table + (key >> c.shift)];
+      if ((u32)p >= (u32)c.n_pages) {
+        p = -1;
+        if (t.err) *t.err = LR_DEV_PAGE_RANGE;
+      }
+    }
+    return p;
+  };
+  auto load_rows = [&](const u8* base, bool value, int length, int tile, int p0, int p1, u32 lds) {
+#pragma unroll
+    for (int i = 0; i < T::LOADS; ++i) {
+      const int r0 = i * T::RPL, half = r0 >> 4, p = half ? p1 : p0;
+      const i32x4_t res = paged_resource(base + paged_offset<T::ROW>(c, p < 0 ? 0 : p, kvh));
+      const int slot = (tile * 32 + half * 16) & ((1 << c.shift) - 1), r = r0 + lrow;
+      const int piece = place ^ (value ? T::v_place(r) : T::k_place(r));
+      const bool ok = p >= 0 && tile * 32 + r < length;
+      paged_load16<true>(res, ok ? lrow * T::ROW + piece * 16 : PAGED_OUT, (slot + (r0 & 15)) * T::ROW, lds + i * 1024);
+    }
+  };
+  // lanes 0..3: the scales of a half's keys, 4..7 of its values
+  auto load_scales = [&](int tile, int p0, int p1) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int p = half ? p1 : p0, slot = (tile * 32 + half * 16) & ((1 << c.shift) - 1);
+      const i32x4_t res = paged_resource(c.scales + paged_scales(c, p < 0 ? 0 : p, kvh));
+      paged_load4(res, p >= 0 && lane < 8 ? (lane >> 2 << c.shift) + (lane & 3) * 4 : PAGED_OUT, slot, lds0 + 2 * T::TILE + half * 256);
+    }
+  };
+  auto load_k = [&](int length, int tile, int p0, int p1) {
+    load_rows(c.k, false, length, tile, p0, p1, lds0);
+    if constexpr (E4M3) load_scales(tile, p0, p1);
+  };
+  auto load_v = [&](int length, int tile, int p0, int p1) { load_rows(c.v, true, length, tile, p0, p1, lds0 + T::TILE); };
+  // (for LDS only: __syncthreads() would wait for the next tiles, too)
+  auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
-    auto load_rows = [&](const u8* base, bool value, int tile, int p0, int p1, u32 lds) {
+  const __amdgpu_buffer_rsrc_t ores = __builtin_amdgcn_make_buffer_rsrc(a.o_part, 0, 0x7fffffff, 0x00020000);
+  const __amdgpu_buffer_rsrc_t mres = __builtin_amdgcn_make_buffer_rsrc(a.ml_part, 0, 0x7fffffff, 0x00020000);
+  auto store_y = [&](int b, int h, int d, const f32x4_t& v, float L) {
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+    u32x2_t out;
+    out.x = pack_bf2(v[0] * inv, v[1] * inv);
+    out.y = pack_bf2(v[2] * inv, v[3] * inv);
+    *reinterpret_cast<u32x2_t*>(a.y + b * a.ldy + (h0 + h) * HD + d) = out;
+  };
+  auto store_part = [&](int part, int h, int d, const f32x4_t& v, float M, float L) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), ores, ((part * 16 + h) * HD + d) * 4, 0, PAGED_COHERENT);
+    if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2_t, f32x2_t{M, L}), mres, (part * 16 + h) * 8, 0, PAGED_COHERENT);
+  };
+  // the sequences of which others have parts, too: one that began before this worker, one that goes on behind it
+  int open_b[2] = {-1, -1}, open_first[2], open_tiles[2];
+  Segment g = segment();
+  if (g.to <= g.from && !next_segment(g)) return;   // (the sequence's cost alone)
+  bf16x8_t qf[KS];
+  load_q(g, qf);
+  int pages = pages_of(g, g.from + wave), p0 = __builtin_amdgcn_readlane(pages, 0), p1 = __builtin_amdgcn_readlane(pages, 1);   // (all of it here by now)
+  if (g.from + wave < g.to) {
+    load_k(g.length, g.from + wave, p0, p1);
+    load_v(g.length, g.from + wave, p0, p1);
+  }
+  for (;;) {
+    // ---- the sequence after this one: its pages and q are asked for now, its first tile when this wave's last one is in registers
+    Segment gn = {};
+    const bool more_sequences = next_segment(gn);
+    int pages_n = -1, pages_next = pages_of(g, g.from + wave + 32 * NW);
+    bf16x8_t qn[KS];
 #pragma unroll
-      for (int i = 0; i < T::LOADS; ++i) {
-        const int r0 = i * T::RPL, half = r0 >> 4, p = half ? p1 : p0;
-        const i32x4_t res = paged_resource(base + paged_offset<T::ROW>(c, p < 0 ? 0 : p, kvh));
-        const int slot = (tile * 32 + half * 16) & ((1 << c.shift) - 1), r = r0 + lrow;
-        const int piece = place ^ (value ? T::v_place(r) : T::k_place(r));
-        const bool ok = p >= 0 && tile * 32 + r < length;
-        paged_load16(res, ok ? lrow * T::ROW + piece * 16 : PAGED_OUT, (slot + (r0 & 15)) * T::ROW, lds + i * 1024);
-      }
-    };
-    // lanes 0..3: the scales of a half's keys, 4..7 of its values
-    auto load_scales = [&](int tile, int p0, int p1) {
+    for (int ks = 0; ks < KS; ++ks) qn[ks] = qf[ks];
+    if (more_sequences) {
+      load_q(gn, qn);
+      pages_n = pages_of(gn, gn.from + wave);
+    }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int p = half ? p1 : p0, slot = (tile * 32 + half * 16) & ((1 << c.shift) - 1);
-        const i32x4_t res = paged_resource(c.scales + paged_scales(c, p < 0 ? 0 : p, kvh));
-        paged_load4(res, p >= 0 && lane < 8 ? (lane >> 2 << c.shift) + (lane & 3) * 4 : PAGED_OUT, slot, lds0 + 2 * T::TILE + half * 256);
-      }
-    };
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qn[ks]));   // (waited for here, together with this sequence's first tile)
+    asm volatile("" : "+v"(pages_n), "+v"(pages_next));
+    const bool next_here = more_sequences && gn.from + wave < gn.to;   // this wave has a tile of it
+    int tile = g.from + wave, j = 0;
+    if (next_here && tile >= g.to) {   // and none of this one
+      p0 = __builtin_amdgcn_readlane(pages_n, 0);
+      p1 = __builtin_amdgcn_readlane(pages_n, 1);
+      load_k(gn.length, gn.from + wave, p0, p1);
+      load_v(gn.length, gn.from + wave, p0, p1);
+    }
 
     f32x4_t o[DT], o_low[E4M3 ? 1 : DT];   // o_low: what the weights' second parts give, apart, since an infinite value times zero is none
 #pragma unroll
@@ -231,26 +313,21 @@ __global__ __launch_bounds__(256, (DecodeTile<HD, E4M3>::PER_CU)) void k_paged_d
       for (int d = 0; d < DT; ++d) o_low[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;   // m: reference point in raw scores; l: this lane's part of the sum
 
-    int p0 = 0, p1 = 0;
-    if (tile < to) {
-      p0 = __builtin_amdgcn_readlane(pages, 0);
-      p1 = __builtin_amdgcn_readlane(pages, 1);
-      load_rows(c.k, false, tile, p0, p1, lds0);
-      if constexpr (E4M3) load_scales(tile, p0, p1);
-      load_rows(c.v, true, tile, p0, p1, lds0 + T::TILE);
-    }
-    while (tile < to) {
-      const int next = tile + 4;
-      const bool more = next < to;
+    while (tile < g.to) {
+      const bool same = tile + NW < g.to, more = same || next_here;
+      const int next = same ? tile + NW : gn.from + wave, next_length = same ? g.length : gn.length;
       int q0 = 0, q1 = 0;
-      if (more) {
+      if (same) {
         if (++j == 32) {
           j = 0;
           pages = pages_next;
-          pages_next = pages_of(next + 128);
+          pages_next = pages_of(g, next + 32 * NW);
         }
         q0 = __builtin_amdgcn_readlane(pages, 2 * j);
         q1 = __builtin_amdgcn_readlane(pages, 2 * j + 1);
+      } else if (next_here) {
+        q0 = __builtin_amdgcn_readlane(pages_n, 0);
+        q1 = __builtin_amdgcn_readlane(pages_n, 1);
       }
       // ---- scores of 2 x 16 keys
       paged_wait_loads<T::LOADS>();
@@ -273,8 +350,7 @@ __global__ __launch_bounds__(256, (DecodeTile<HD, E4M3>::PER_CU)) void k_paged_d
         }
         if (more) {
           paged_wait_lds();
-          load_rows(c.k, false, next, q0, q1, lds0);
-          if constexpr (E4M3) load_scales(next, q0, q1);
+          load_k(next_length, next, q0, q1);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -298,7 +374,7 @@ __global__ __launch_bounds__(256, (DecodeTile<HD, E4M3>::PER_CU)) void k_paged_d
         }
       }
       // element e of half h: key 16 h + 4 l4 + e of the tile, head l16
-      const int there = length - tile * 32;
+      const int there = g.length - tile * 32;
       if (there < 32 || (p0 | p1) < 0) {   // uniform
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -360,7 +436,7 @@ __global__ __launch_bounds__(256, (DecodeTile<HD, E4M3>::PER_CU)) void k_paged_d
       }
       if (more) {
         paged_wait_lds();
-        load_rows(c.v, true, next, q0, q1, lds0 + T::TILE);
+        load_v(next_length, next, q0, q1);
       }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
@@ -379,14 +455,16 @@ __global__ __launch_bounds__(256, (DecodeTile<HD, E4M3>::PER_CU)) void k_paged_d
         f32x4_t& to_low = E4M3 ? o[d] : o_low[E4M3 ? 0 : d];
         to_low = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[d], __builtin_bit_cast(bf16x8_t, pl), to_low, 0, 0, 0);
       }
-      tile = next;
+      tile = same ? next : g.to;
       p0 = q0;
       p1 = q1;
     }
 
-    // ---- the four waves' results together (each in its own LDS, where nothing is on its way any more)
+    // ---- the waves' results together
     l = rows_sum(l);
-    float* const my_o = reinterpret_cast<float*>(mine);
+    float* const results = reinterpret_cast<float*>(paged_lds + NW * T::WAVE);
+    float* const my_o = results + wave * (T::RESULT / 4);
+    barrier();   // (nobody reads the sequence's before any more)
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       f32x4_t v = o[d];
@@ -396,116 +474,140 @@ __global__ __launch_bounds__(256, (DecodeTile<HD, E4M3>::PER_CU)) void k_paged_d
       *reinterpret_cast<f32x4_t*>(my_o + l16 * T::LDO + d * 16 + l4 * 4) = v;
     }
     if (l4 == 0) s_ml[wave][l16][0] = m * c2, s_ml[wave][l16][1] = l;   // (from here on in powers of two)
-    __syncthreads();
-    const bool whole = from == 0 && to == n_tiles;
-    const int slot = (group * (int)gridDim.x + w) * 2 + (from == 0 ? 1 : 0);
-    const __amdgpu_buffer_rsrc_t ores = __builtin_amdgcn_make_buffer_rsrc(a.o_part, 0, 0x7fffffff, 0x00020000);
-    const __amdgpu_buffer_rsrc_t mres = __builtin_amdgcn_make_buffer_rsrc(a.ml_part, 0, 0x7fffffff, 0x00020000);
-    u16* const y = a.y + b * a.ldy + h0 * HD;
-    auto store_y = [&](int h, int d, const f32x4_t& v, float L) {
-      const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-      u32x2_t out;
-      out.x = pack_bf2(v[0] * inv, v[1] * inv);
-      out.y = pack_bf2(v[2] * inv, v[3] * inv);
-      *reinterpret_cast<u32x2_t*>(y + h * HD + d) = out;
-    };
-    auto store_part = [&](int part, int h, int d, const f32x4_t& v, float M, float L) {
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), ores, ((part * 16 + h) * HD + d) * 4, 0, PAGED_COHERENT);
-      if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2_t, f32x2_t{M, L}), mres, (part * 16 + h) * 8, 0, PAGED_COHERENT);
-    };
-    for (int i = tid; i < nh * (HD / 4); i += 256) {
+    barrier();
+    const bool whole = g.from == 0 && g.to == g.n_tiles;
+    const int slot = (group * (int)gridDim.x + w) * 2 + (g.from == 0 ? 1 : 0);
+    for (int i = tid; i < nh * (HD / 4); i += 64 * NW) {
       const int h = i / (HD / 4), d = i % (HD / 4) * 4;
       float M = s_ml[0][h][0], L = 0.0f;
 #pragma unroll
-      for (int k = 1; k < 4; ++k) M = fmaxf(M, s_ml[k][h][0]);
+      for (int k = 1; k < NW; ++k) M = fmaxf(M, s_ml[k][h][0]);
       // (a wave that has seen no key has -inf, 0, 0; one that has seen only NaN -inf, NaN, NaN)
       const float ref = M == -INFINITY ? 0.0f : M;
       f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < NW; ++k) {
         const float f = exp2_hw(s_ml[k][h][0] - ref);
         L += f * s_ml[k][h][1];
-        v += f * *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(paged_lds + k * T::WAVE) + h * T::LDO + d);
+        v += f * *reinterpret_cast<const f32x4_t*>(results + k * (T::RESULT / 4) + h * T::LDO + d);
       }
-      if (whole) store_y(h, d, v, L);
+      if (whole) store_y(g.b, h, d, v, L);
       else store_part(slot, h, d, v, M, L);
     }
     if (!whole) {
-      // Workers w0 .. w1 have parts of this sequence.  Those of one block of PAGED_BLOCK workers are put together by the block's last, the
-      // blocks' results by the last block's.
-      const auto worker = [&](int tile) { return (int)((((int64_t)tile + 1) * workers - 1) / total); };
-      const int w0 = worker(first), w1 = worker(first + n_tiles - 1), k0 = w0 / PAGED_BLOCK, k1 = w1 / PAGED_BLOCK, kw = w / PAGED_BLOCK;
-      const int n_blocks = (gridDim.x + PAGED_BLOCK - 1) / PAGED_BLOCK;
-      const auto part_of = [&](int x) { return (group * (int)gridDim.x + x) * 2 + (x == w0 ? 1 : 0); };
-      const auto block_of = [&](int k) { return (group * n_blocks + k) * 2 + (k == k0 ? 1 : 0); };
-      const int block_parts = gridDim.y * gridDim.x * 2;
-      // true in the last of n workers: then all others' results can be read
-      auto last_of = [&](u32* ticket, int n) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (tid == 0) {
-          const u32 was = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          if (was + 1 == (u32)n) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          *s_ticket = was + 1;
-        }
-        __syncthreads();
-        const bool last = *s_ticket == (u32)n;
-        asm volatile("" ::: "memory");
-        return last;
-      };
-      // parts u0 .. u1, at places(u), into y or the place `out`
-      auto together = [&](int u0, int u1, auto places, int out) {
-        for (int i = tid; i < nh * (HD / 4); i += 256) {
-          const int h = i / (HD / 4), d = i % (HD / 4) * 4;
-          float M = -INFINITY, L = 0.0f;
-          f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-          for (int u = u0; u <= u1; u += 8) {
-            f32x4_t ov[8];
-            f32x2_t ml[8];
+      const int i = g.from == 0;
+      open_b[i] = g.b;
+      open_first[i] = g.first;
+      open_tiles[i] = g.n_tiles;
+    }
+    if (!more_sequences) break;
+    g = gn;
+    pages = pages_n;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {   // (all of them on their way before the first is used)
-              const int from_ = u + k <= u1 ? places(u + k) * 16 + h : -1;
-              ov[k] = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ores, from_ < 0 ? PAGED_OUT : (from_ * HD + d) * 4, 0, PAGED_COHERENT));
-              ml[k] = __builtin_bit_cast(f32x2_t, __builtin_amdgcn_raw_buffer_load_b64(mres, from_ < 0 ? PAGED_OUT : from_ * 8, 0, PAGED_COHERENT));
-            }
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = qn[ks];
+  }
+
+  // ---- parts put together (at the end: the stream above waits for nobody).  Workers w0 .. w1 have parts of a sequence; those of one block of
+  // PAGED_BLOCK workers are put together by the block's last, the blocks' results by the last block's.
+  const int n_blocks = (gridDim.x + PAGED_BLOCK - 1) / PAGED_BLOCK, kw = w / PAGED_BLOCK, block_parts = 2 * (int)(gridDim.y * gridDim.x);
+  const auto worker = [&](int place) {
+    const int n = larger * (each + 1);
+    return (int)(place < n ? (u32)place / (u32)(each + 1) : larger + (u32)(place - n) / (u32)each);
+  };
+  // workers' parts first (of a block, or all of them where they are one block's), then blocks'; part u lies at places + 2 u, + 1 for the one
+  // with the sequence's first tile
+  struct Open {
+    u32* ticket;
+    int u0, u1, places, began, n_parts;
+  };
+  int k0[2] = {}, k1[2] = {};
+  auto workers_of = [&](int i) {
+    Open p = {};
+    if (open_b[i] < 0) return p;
+    const int w0 = worker(open_first[i]), w1 = worker(open_first[i] + open_tiles[i] - 1);
+    k0[i] = w0 / PAGED_BLOCK;
+    k1[i] = w1 / PAGED_BLOCK;
+    const bool one = k0[i] == k1[i];
+    p.u0 = one ? w0 : max(w0, kw * PAGED_BLOCK);
+    p.u1 = one ? w1 : min(w1, kw * PAGED_BLOCK + PAGED_BLOCK - 1);
+    p.places = group * (int)gridDim.x * 2;
+    p.began = w0;
+    p.ticket = a.tickets + (one ? (int64_t)group * t.B + open_b[i] : (int64_t)gridDim.y * t.B + (group * n_blocks + kw) * 2 + (kw == k0[i]));
+    p.n_parts = p.u1 - p.u0 + 1;
+    return p;
+  };
+  // s_ticket[i] = how many of p's parts there are with this one; then, in the last worker, all others' results can be read
+  auto count = [&](const Open& p, int i) {
+    if (tid == 64 * i && p.n_parts) {
+      const u32 was = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (was + 1 == (u32)p.n_parts) __hip_atomic_store(p.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_ticket[i] = was + 1;
+    }
+  };
+  if (open_b[0] < 0 && open_b[1] < 0) return;
+  Open both[2] = {workers_of(0), workers_of(1)};
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  barrier();
+  count(both[0], 0);
+  count(both[1], 1);
+  barrier();
+  const bool last0 = both[0].n_parts && s_ticket[0] == (u32)both[0].n_parts, last1 = both[1].n_parts && s_ticket[1] == (u32)both[1].n_parts;
+  asm volatile("" ::: "memory");
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    bool last = i ? last1 : last0;
+    Open p = i ? both[1] : both[0];
+    const int b = i ? open_b[1] : open_b[0], first_block = i ? k0[1] : k0[0], last_block = i ? k1[1] : k1[0];
+    bool final = first_block == last_block;
+    const int block = (group * n_blocks + kw) * 2 + (kw == first_block ? 1 : 0);
+#pragma unroll 1
+    while (last) {
+#pragma unroll 1
+      for (int x = tid; x < nh * (HD / 4); x += 64 * NW) {
+        const int h = x / (HD / 4), d = x % (HD / 4) * 4;
+        float M = -INFINITY, L = 0.0f;
+        f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+        for (int u = p.u0; u <= p.u1; u += PAGED_BLOCK) {
+          f32x4_t ov[PAGED_BLOCK];
+          f32x2_t ml[PAGED_BLOCK];
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (u + k <= u1) {
-                const float Mn = fmaxf(M, ml[k][0]), ref = Mn == -INFINITY ? 0.0f : Mn;
-                const float f0 = exp2_hw(M - ref), f1 = exp2_hw(ml[k][0] - ref);
-                L = L * f0 + ml[k][1] * f1;
-                v = v * f0 + ov[k] * f1;
-                M = Mn;
-              }
+          for (int k = 0; k < PAGED_BLOCK; ++k) {   // (all of them on their way before the first is used)
+            const int from = (p.places + 2 * (u + k) + (u + k == p.began ? 1 : 0)) * 16 + h;
+            ml[k] = __builtin_bit_cast(f32x2_t, __builtin_amdgcn_raw_buffer_load_b64(mres, u + k <= p.u1 ? from * 8 : PAGED_OUT, 0, PAGED_COHERENT));
+            ov[k] = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ores, u + k <= p.u1 ? (from * HD + d) * 4 : PAGED_OUT, 0, PAGED_COHERENT));
           }
-          if (out < 0) store_y(h, d, v, L);
-          else store_part(out, h, d, v, M, L);
+          float top = M;
+#pragma unroll
+          for (int k = 0; k < PAGED_BLOCK; ++k) {
+            ml[k][0] = u + k <= p.u1 ? ml[k][0] : -INFINITY;   // (what is not there: weight, sum and values zero)
+            top = fmaxf(top, ml[k][0]);
+          }
+          const float ref = top == -INFINITY ? 0.0f : top, f0 = exp2_hw(M - ref);
+          L *= f0;
+          v *= f0;
+          M = top;
+#pragma unroll
+          for (int k = 0; k < PAGED_BLOCK; ++k) {
+            const float f = exp2_hw(ml[k][0] - ref);
+            L = fmaf(f, ml[k][1], L);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = fmaf(f, ov[k][e], v[e]);
+          }
         }
-      };
-      u32* const own = a.tickets + (int64_t)group * t.B + b;
-      if (k0 == k1) {
-        if (last_of(own, w1 - w0 + 1)) together(w0, w1, part_of, -1);
-      } else {
-        u32* const blocks = a.tickets + (int64_t)gridDim.y * t.B + block_of(kw);
-        const int u0 = max(w0, kw * PAGED_BLOCK), u1 = min(w1, kw * PAGED_BLOCK + PAGED_BLOCK - 1);
-        if (last_of(blocks, u1 - u0 + 1)) {
-          together(u0, u1, part_of, block_parts + block_of(kw));
-          if (last_of(own, k1 - k0 + 1)) together(k0, k1, [&](int k) { return block_parts + block_of(k); }, -1);
-        }
+        if (final) store_y(b, h, d, v, L);
+        else store_part(block_parts + block, h, d, v, M, L);
       }
+      if (final) break;
+      final = true;
+      p = {a.tickets + (int64_t)group * t.B + b, first_block, last_block, block_parts + group * n_blocks * 2, first_block, last_block - first_block + 1};
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      barrier();
+      count(p, 0);
+      barrier();
+      last = s_ticket[0] == (u32)p.n_parts;
+      asm volatile("" ::: "memory");
     }
-    __syncthreads();
-    // ---- on to the next sequence that has tiles
-    at = first + to;
-    if (at >= end) return;
-    first += n_tiles;
-    unsigned long long others = __ballot(tiles > 0) & (s == 63 ? 0ull : ~0ull << (s + 1));
-    while (!others) {
-      if (b0 + 64 >= t.B) return;   // (never: there are tiles left)
-      look(b0 + 64);
-      others = __ballot(tiles > 0);
-    }
-    s = __builtin_ctzll(others);
   }
 }
 
@@ -543,7 +645,7 @@ static int launch_paged_decode(const PagedCache& c, const PagedBatch& t, const P
   constexpr size_t lds = DecodeTile<HD, E4M3>::LDS;
   static std::atomic<unsigned long long> raised{0};
   if (!lr_raise_lds_limit(reinterpret_cast<const void*>(&k_paged_decode<HD, E4M3>), lds, raised)) return LR_E_LAUNCH;
-  k_paged_decode<HD, E4M3><<<dim3(p.workers, p.groups), dim3(256), lds, s>>>(c, t, a);
+  k_paged_decode<HD, E4M3><<<dim3(p.workers, p.groups), dim3(64 * DecodeTile<HD, E4M3>::NW), lds, s>>>(c, t, a);
   return lr_launch_status();
 }
 
@@ -584,12 +686,7 @@ __device__ __forceinline__ bool prompt_block(const PagedCache& c, const PagedBat
     n = i < t.B ? t.starts[i + 1] - start : 0;
     n = start < 0 || start > rows || n < 0 ? 0 : min(n, rows - start);
     blocks = (int)(((int64_t)n * G + PROMPT_ROWS - 1) / PROMPT_ROWS);
-    upto = blocks;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(upto, o, 64);
-      upto += lane >= o ? u : 0;
-    }
+    upto = paged_sums(blocks);
     return __builtin_amdgcn_readlane(upto, 63);
   };
   for (int i = 0; i < t.B; i += 64) total += look(i);

@@ -36,6 +36,19 @@ __device__ __forceinline__ int paged_sequence(const PagedBatch& t, int row) {
   return b;
 }
 
+// Inclusive sums over a wave's lanes, on the vector unit.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int paged_dpp0(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int paged_sums(int v) {
+  v += paged_dpp0<0x111, 0xf>(v);   // row_shr:1, 2, 4, 8: within 16 lanes
+  v += paged_dpp0<0x112, 0xf>(v);
+  v += paged_dpp0<0x114, 0xf>(v);
+  v += paged_dpp0<0x118, 0xf>(v);
+  v += paged_dpp0<0x142, 0xa>(v);   // row_bcast:15: lane 15 to row 1, 47 to row 3
+  v += paged_dpp0<0x143, 0xc>(v);   // row_bcast:31: to rows 2 and 3
+  return v;
+}
+
 // Bytes from the start of k, v to (page, kv head, slot 0)
 template <int ROW>
 __device__ __forceinline__ int64_t paged_offset(const PagedCache& c, int page, int head) {
@@ -70,7 +83,7 @@ static inline int paged_arguments(const lr_paged_cache_t* cache, const lr_paged_
   if (cache->page < 16 || cache->page > 256 || (cache->page & (cache->page - 1))) return LR_E_UNSUPPORTED;
   // (positions, and tiles of 32 keys of all sequences, are 32-bit numbers)
   const int64_t most = (int64_t)batch->pages * cache->page;
-  if (batch->B > 65535 || most > (1 << 30) || batch->B * (most / 32 + 1) >= 0x7fffffff) return LR_E_UNSUPPORTED;
+  if (batch->B > 65535 || most > (1 << 30) || batch->B * (most / 32 + 8) >= 0x7fffffff) return LR_E_UNSUPPORTED;
   c.k = (u8*)cache->k;
   c.v = (u8*)cache->v;
   c.scales = (u8*)cache->scales;

@@ -65,7 +65,7 @@ class PagedBatch:
 
     def __init__(self, cache: "PagedKVCache", table: Tensor, lengths: Tensor, n_head: int, starts: Optional[Tensor], rows: int):
         self.table, self.lengths, self.starts, self.n_head, self.rows = table, lengths, starts, n_head, rows
-        self.shape = cache.shape
+        self.shape, self.device = cache.shape, table.device
         self.desc = _hip.paged_batch_desc(table, lengths, starts)
         need = _hip.paged_attention_scratch_bytes(cache.desc(), self.desc, rows, n_head)
         if need == 0:
@@ -102,14 +102,23 @@ class PagedKVCache(nn.Module):
         self.register_buffer("scales", scales)
         self._desc = None
 
+    def __setattr__(self, name, value):
+        super().__setattr__(name, value)
+        if name in ("k_pages", "v_pages", "scales"):
+            self._desc = None
+
+    def __getstate__(self):
+        return dict(self.__dict__, _desc=None)     # (addresses are this process's and this object's)
+
     @property
     def shape(self):
-        return tuple(self.k_pages.shape[1:])
+        """(kv heads, page, head_dim, type): a batch serves caches of the same."""
+        return (*self.k_pages.shape[1:], self.k_pages.dtype)
 
     def desc(self):
         if self._desc is None:
             self._desc = _hip.paged_cache_desc(self.k_pages, self.v_pages, self.scales)
-            self._device = self.k_pages.device
+            self._device, self._shape = self.k_pages.device, self.shape
         return self._desc
 
     def _apply(self, fn, recurse=True):
@@ -127,9 +136,10 @@ class PagedKVCache(nn.Module):
         return PagedBatch(self, table, lengths, n_head, starts, table.shape[0] if rows is None else rows)
 
     def _check(self, batch: PagedBatch, rows: int):
-        desc = self.desc()
-        if batch.shape != self.shape or rows > batch.rows:
-            raise ValueError(f"a batch for up to {batch.rows} rows and pages {batch.shape}: got {rows} rows, pages {self.shape}")
+        desc = self._desc or self.desc()
+        if batch.shape != self._shape or rows > batch.rows or batch.device != self._device:
+            raise ValueError(f"a batch for up to {batch.rows} rows and pages {batch.shape} on {batch.device}: got {rows} rows, pages {self._shape} "
+                             f"on {self._device}")
         return desc
 
     def write(self, batch: PagedBatch, qkv: Tensor, q: Tensor, rope: Optional[Tensor] = None, interleaved: bool = True) -> Tensor:
