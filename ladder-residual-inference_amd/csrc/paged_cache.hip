@@ -4,39 +4,48 @@
 // reads (where the row belongs, then its page).  A lane has 8 elements of a head's row (16 bytes of bf16), HD / 8 lanes a row.
 #include "paged_common.h"
 
-constexpr int PAGED_TOKENS = 4;   // of a workgroup, at most
+constexpr int PAGED_TOKENS = 16;   // of a workgroup, at most
+constexpr int PAGED_AHEAD = 4;     // rows that a lane asks for before it works on the first
 
-// Where a workgroup's tokens belong: sequence, position, page; one wave per token.  page -1: the token is left alone.
+// Where a workgroup's tokens belong.  page -1: the token is left alone.
 struct PagedPlace {
   int pos[PAGED_TOKENS], page[PAGED_TOKENS];
 };
 // `limit`: positions from there on have no angle.  A token behind the last sequence, or an empty place of a batch, has no place and is no
-// error; a position or a page that is out of range is one.
+// error; a position or a page that is out of range is one.  A wave looks after every fourth token, and lane j of it after its j-th.
 __device__ __forceinline__ void paged_places(const PagedCache& c, const PagedBatch& t, int row0, int rows, int tokens, int limit, PagedPlace& at) {
-  const int wave = threadIdx.x >> 6;
-  if (wave < tokens) {
-    const int row = row0 + wave;
-    int page = -1, pos = 0;
-    if (row < rows) {
-      int b = row, end = row + 1;
-      if (t.starts) {
-        b = paged_sequence(t, row);
-        end = b < t.B ? t.starts[b + 1] : 0;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int i = wave + 4 * lane, row = row0 + i;
+  int b = row;
+  if (t.starts) {
+    b = 0;
+    for (int i0 = 0; i0 < t.B; i0 += 64) {   // as many sequences as have ended by then: 64 of them at a time
+      const int end = i0 + lane < t.B ? t.starts[i0 + lane + 1] : 0x7fffffff;
+      int most = 0;
+      for (int j = 0; wave + 4 * j < tokens; ++j) {
+        const int n = __popcll(__ballot(end <= row0 + wave + 4 * j));
+        if (lane == j) b += n;
+        most = n > most ? n : most;
       }
-      if (b < t.B) {
-        const int length = t.lengths[b];
-        pos = length - (end - row);
-        int code = 0;
-        if (pos < 0 || pos >> c.shift >= t.pages || pos >= limit) {
-          code = t.starts || length != 0 ? LR_DEV_POS_RANGE : 0;
-        } else {
-          page = t.table[(int64_t)b * t.ld_table + (pos >> c.shift)];
-          if (page < 0 || page >= c.n_pages) code = LR_DEV_PAGE_RANGE, page = -1;
-        }
-        if (code && t.err && (threadIdx.x & 63) == 0) *t.err = code;
-      }
+      if (most < 64) break;
     }
-    if ((threadIdx.x & 63) == 0) at.pos[wave] = pos, at.page[wave] = page;
+  }
+  if (i < tokens) {
+    int page = -1, pos = 0;
+    if (row < rows && b < t.B) {
+      const int length = t.lengths[b];
+      pos = length - ((t.starts ? t.starts[b + 1] : row + 1) - row);
+      int code = 0;
+      if (pos < 0 || pos >> c.shift >= t.pages || pos >= limit) {
+        code = t.starts || length != 0 ? LR_DEV_POS_RANGE : 0;
+      } else {
+        page = t.table[(int64_t)b * t.ld_table + (pos >> c.shift)];
+        if (page < 0 || page >= c.n_pages) code = LR_DEV_PAGE_RANGE, page = -1;
+      }
+      if (code && t.err) *t.err = code;
+    }
+    at.pos[i] = pos;
+    at.page[i] = page;
   }
   __syncthreads();
 }
@@ -106,37 +115,50 @@ __global__ __launch_bounds__(256) void k_paged_write(const PagedCache c, const P
   const int row0 = blockIdx.x * w.tokens;
   paged_places(c, t, row0, w.rows, w.tokens, w.rope ? w.rope_len : 0x7fffffff, at);
   constexpr int LANES = HD / 8, ROWS = 256 / LANES;
-  const int heads = w.Hq + 2 * c.Hkv, d = threadIdx.x % LANES * 8;
-  for (int i = threadIdx.x / LANES; i < w.tokens * heads; i += ROWS) {   // (all lanes of a row go round together)
-    const int token = i / heads, head = i - token * heads, page = at.page[token];
-    if (page < 0) continue;
-    const int pos = at.pos[token];
-    const u16* const row = w.x + (row0 + token) * w.ldx + head * HD;
-    float f[8];
-    unpack8(ld16(row + d), f);
-    if (w.rope && head < w.Hq + c.Hkv && d < w.rot) paged_turn<PAIRS>(f, row, d, (const T*)w.rope + (int64_t)pos * w.rot, w.rot);
-    if (head < w.Hq) {
-      st16(w.q + (row0 + token) * w.ldq + head * HD + d, pack8(f));
-      continue;
+  const int heads = w.Hq + 2 * c.Hkv, d = threadIdx.x % LANES * 8, n = w.tokens * heads;
+  for (int i0 = threadIdx.x / LANES; i0 < n; i0 += ROWS * PAGED_AHEAD) {   // (all lanes of a row go round together)
+    uint4 x[PAGED_AHEAD];
+#pragma unroll
+    for (int u = 0; u < PAGED_AHEAD; ++u) {
+      const int i = i0 + u * ROWS < n ? i0 + u * ROWS : i0, token = i / heads, head = i - token * heads;
+      x[u] = ld16_once(w.x + (at.page[token] >= 0 ? row0 + token : 0) * w.ldx + head * HD + d);
     }
-    const int value = head >= w.Hq + c.Hkv, kvh = head - w.Hq - value * c.Hkv, slot = pos & ((1 << c.shift) - 1);
-    u8* const to = (value ? c.v : c.k) + paged_offset<HD * (E4M3 ? 1 : 2)>(c, page, kvh);
-    if constexpr (!E4M3) {
-      st16(to + (slot * HD + d) * 2, pack8(f));
-    } else {
-      float amax = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(f[j]) < INFINITY ? fabsf(f[j]) : 0.0f);
-      amax = row_max<HD>(amax);
-      const u32 byte = paged_exponent(amax);
-      const float inv = paged_inverse(byte);
+    for (int u = 0; u < PAGED_AHEAD; ++u) {
+      const int i = i0 + u * ROWS;
+      if (i >= n) break;
+      const int token = i / heads, head = i - token * heads, page = at.page[token];
+      if (page < 0) continue;
+      const int pos = at.pos[token];
+      float f[8];
+      unpack8(x[u], f);
+      if (w.rope && head < w.Hq + c.Hkv && d < w.rot)
+        paged_turn<PAIRS>(f, w.x + (row0 + token) * w.ldx + head * HD, d, (const T*)w.rope + (int64_t)pos * w.rot, w.rot);
+      if (head < w.Hq) {
+        // (qkv and q non-temporal: 26.7 -> 24.4 us of those prompts.  k and v are not: 23.2, but the attention behind it 16 us longer)
+        const uint4 o = pack8(f);
+        __builtin_nontemporal_store(u32x4_t{o.x, o.y, o.z, o.w}, reinterpret_cast<u32x4_t*>(w.q + (row0 + token) * w.ldq + head * HD + d));
+        continue;
+      }
+      const int value = head >= w.Hq + c.Hkv, kvh = head - w.Hq - value * c.Hkv, slot = pos & ((1 << c.shift) - 1);
+      u8* const to = (value ? c.v : c.k) + paged_offset<HD * (E4M3 ? 1 : 2)>(c, page, kvh);
+      if constexpr (!E4M3) {
+        st16(to + (slot * HD + d) * 2, pack8(f));
+      } else {
+        float amax = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = fabsf(f[j]) < INFINITY ? f[j] * inv : NAN;   // (e4m3 has no infinities)
-      u32x2_t o;
-      o.x = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false), true);
-      o.y = __builtin_amdgcn_cvt_pk_fp8_f32(f[6], f[7], __builtin_amdgcn_cvt_pk_fp8_f32(f[4], f[5], 0, false), true);
-      *reinterpret_cast<u32x2_t*>(to + slot * HD + d) = o;
-      if (d == 0) c.scales[paged_scales(c, page, kvh) + (value << c.shift) + slot] = (u8)byte;
+        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(f[j]) < INFINITY ? fabsf(f[j]) : 0.0f);
+        amax = row_max<HD>(amax);
+        const u32 byte = paged_exponent(amax);
+        const float inv = paged_inverse(byte);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = fabsf(f[j]) < INFINITY ? f[j] * inv : NAN;   // (e4m3 has no infinities)
+        u32x2_t o;
+        o.x = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false), true);
+        o.y = __builtin_amdgcn_cvt_pk_fp8_f32(f[6], f[7], __builtin_amdgcn_cvt_pk_fp8_f32(f[4], f[5], 0, false), true);
+        *reinterpret_cast<u32x2_t*>(to + slot * HD + d) = o;
+        if (d == 0) c.scales[paged_scales(c, page, kvh) + (value << c.shift) + slot] = (u8)byte;
+      }
     }
   }
 }
@@ -153,31 +175,50 @@ __global__ __launch_bounds__(256) void k_paged_read(const PagedCache c, const Pa
   const int row0 = blockIdx.x * r.tokens;
   paged_places(c, t, row0, r.rows, r.tokens, 0x7fffffff, at);
   constexpr int LANES = HD / 8, ROWS = 256 / LANES;
-  const int d = threadIdx.x % LANES * 8;
-  for (int i = threadIdx.x / LANES; i < r.tokens * 2 * c.Hkv; i += ROWS) {
-    const int token = i / (2 * c.Hkv), j = i - token * 2 * c.Hkv, value = j >= c.Hkv, kvh = j - value * c.Hkv, page = at.page[token];
-    if (page < 0) continue;
-    const int slot = at.pos[token] & ((1 << c.shift) - 1);
-    const u8* const from = (value ? c.v : c.k) + paged_offset<HD * (E4M3 ? 1 : 2)>(c, page, kvh);
-    uint4 o;
-    if constexpr (!E4M3) {
-      o = ld16(from + (slot * HD + d) * 2);
-    } else {
-      const u32x2_t raw = *reinterpret_cast<const u32x2_t*>(from + slot * HD + d);
-      const float s = paged_scale(c.scales[paged_scales(c, page, kvh) + (value << c.shift) + slot]);
-      o.x = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.x, s, false));
-      o.y = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.x, s, true));
-      o.z = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.y, s, false));
-      o.w = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.y, s, true));
+  const int d = threadIdx.x % LANES * 8, n = r.tokens * 2 * c.Hkv;
+  for (int i0 = threadIdx.x / LANES; i0 < n; i0 += ROWS * PAGED_AHEAD) {
+    uint4 x[PAGED_AHEAD];   // (e4m3: eight bytes)
+    u32 byte[PAGED_AHEAD];
+#pragma unroll
+    for (int u = 0; u < PAGED_AHEAD; ++u) {
+      const int i = i0 + u * ROWS < n ? i0 + u * ROWS : i0, token = i / (2 * c.Hkv), j = i - token * 2 * c.Hkv, value = j >= c.Hkv, kvh = j - value * c.Hkv;
+      const int page = at.page[token] < 0 ? 0 : at.page[token], slot = at.page[token] < 0 ? 0 : at.pos[token] & ((1 << c.shift) - 1);
+      const u8* const from = (value ? c.v : c.k) + paged_offset<HD * (E4M3 ? 1 : 2)>(c, page, kvh);
+      if constexpr (!E4M3) {
+        x[u] = ld16(from + (slot * HD + d) * 2);
+      } else {
+        const u32x2_t raw = *reinterpret_cast<const u32x2_t*>(from + slot * HD + d);
+        x[u].x = raw.x;
+        x[u].y = raw.y;
+        byte[u] = c.scales[paged_scales(c, page, kvh) + (value << c.shift) + slot];
+      }
     }
-    st16((value ? r.v + (row0 + token) * r.ldv : r.k + (row0 + token) * r.ldk) + kvh * HD + d, o);
+#pragma unroll
+    for (int u = 0; u < PAGED_AHEAD; ++u) {
+      const int i = i0 + u * ROWS;
+      if (i >= n) break;
+      const int token = i / (2 * c.Hkv), j = i - token * 2 * c.Hkv, value = j >= c.Hkv, kvh = j - value * c.Hkv;
+      if (at.page[token] < 0) continue;
+      uint4 o = x[u];
+      if constexpr (E4M3) {
+        const float s = paged_scale(byte[u]);
+        o.x = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[u].x, s, false));
+        o.y = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[u].x, s, true));
+        o.z = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[u].y, s, false));
+        o.w = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[u].y, s, true));
+      }
+      // (non-temporal: 16 sequences of the 8B model from e4m3, 116 MB, 27.5 -> 21.2 us)
+      u16* const to = (value ? r.v + (row0 + token) * r.ldv : r.k + (row0 + token) * r.ldk) + kvh * HD + d;
+      __builtin_nontemporal_store(u32x4_t{o.x, o.y, o.z, o.w}, reinterpret_cast<u32x4_t*>(to));
+    }
   }
 }
 
-// Tokens of a workgroup: as many as give every lane something, the grid no fewer workgroups than the chip holds at once.
-static inline int paged_tokens(int rows, int heads, int hd) {
-  const int fill = 256 / (hd / 8) / heads, spread = rows / (8 * 256);
-  const int n = fill > spread ? spread : fill;
+// Tokens of a workgroup, which share the search for their places: as many as leave each of 256 CUs so many workgroups.  us, 6 prompts of the 8B
+// model into e4m3 with 4 and with 1 token: 28.3, 26.7 (48 rows of q, k and v per token); 16 sequences of it read back with 16, 9 and 4: 27.5,
+// 27.5, 29.2 (16 rows).
+static inline int paged_tokens(int rows, int per_cu) {
+  const int n = rows / (per_cu * 256);
   return n < 1 ? 1 : n > PAGED_TOKENS ? PAGED_TOKENS : n;
 }
 
@@ -201,7 +242,7 @@ extern "C" int lr_paged_write(const lr_paged_cache_t* cache, const lr_paged_batc
   if (ldqkv % 8 || ldq % 8) return LR_E_ALIGN;
   if (rope && (rope_len <= 0 || rot <= 0 || rot > hd)) return LR_E_SHAPE;
   if (rope && (rot % 16 || (rope_dtype != LR_BF16 && rope_dtype != LR_F32))) return LR_E_UNSUPPORTED;
-  const int tokens = paged_tokens(rows, Hq + 2 * c.Hkv, hd);
+  const int tokens = paged_tokens(rows, 32);
   const PagedWrite w = {(const u16*)qkv, ldqkv, (u16*)q, ldq, rope, rope_len, rot, rows, Hq, tokens};
   const unsigned grid = (unsigned)((rows + tokens - 1) / tokens);
   const bool f32 = rope_dtype == LR_F32;
@@ -226,7 +267,7 @@ extern "C" int lr_paged_read(const lr_paged_cache_t* cache, const lr_paged_batch
   if (rows <= 0 || (t.starts == nullptr && rows != t.B) || c.Hkv > 65535) return LR_E_SHAPE;
   if (ldk < (int64_t)c.Hkv * hd || ldv < (int64_t)c.Hkv * hd) return LR_E_SHAPE;
   if (ldk % 8 || ldv % 8) return LR_E_ALIGN;
-  const int tokens = paged_tokens(rows, 2 * c.Hkv, hd);
+  const int tokens = paged_tokens(rows, 4);
   const PagedRead r = {(u16*)k, (u16*)v, ldk, ldv, rows, tokens};
   const dim3 grid((unsigned)((rows + tokens - 1) / tokens));
   hipStream_t s = (hipStream_t)stream;

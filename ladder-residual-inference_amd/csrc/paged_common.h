@@ -23,19 +23,6 @@ __device__ __forceinline__ int paged_length(const PagedBatch& t, int shift, int 
   return n < 0 ? 0 : n > most ? most : n;
 }
 
-// The sequence that a row of the call belongs to: as many as have ended by then.  By all lanes of a wave, 64 of them at a time (a
-// binary search is a chain of memory round trips).  B: the row is behind the last one's.
-__device__ __forceinline__ int paged_sequence(const PagedBatch& t, int row) {
-  const int lane = threadIdx.x & 63;
-  int b = 0;
-  for (int i = 0; i < t.B; i += 64) {
-    const int n = __popcll(__ballot(i + lane < t.B && t.starts[i + lane + 1] <= row));
-    b += n;
-    if (n < 64) break;   // (starts ascend)
-  }
-  return b;
-}
-
 // Inclusive sums over a wave's lanes, on the vector unit.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int paged_dpp0(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
