@@ -654,9 +654,8 @@ static int launch_paged_decode(const PagedCache& c, const PagedBatch& t, const P
 // a wave 32, whatever G is: the columns of the products
 //   S^T[key][row] = K q^T,   O^T[dim][row] += V^T P^T
 // on the matrix cores (32x32x16).  A column is a lane, so maxima, sums and factors are a lane's own, and the 16 scores that it holds of 32 keys are, in
-// their order, the second product's operand.  Weights enter as bf16 and so they do the sum that divides them: y is off by the weights'
-// rounding, 2^-9 of each at random, about as much as y's own rounding (1.41 times the error of y rounded from exact sums, where keys
-// are many).  Keys come 64 at a time into one of two buffers, one barrier per 64; bf16 by loads straight into LDS, e4m3 through registers, expanded on
+// their order, the second product's operand.  Weights enter as one bf16 number: y is off by their rounding, at most 2^-8 of each and at random,
+// where keys are many about as much as by y's own rounding (1.41 times the error of exact sums rounded).  Keys come 64 at a time into one of two buffers, one barrier per 64; bf16 by loads straight into LDS, e4m3 through registers, expanded on
 // the way with its row's power of two: from there on the two are the same.
 // Few rows: a workgroup's keys are cut among several, whose results a second launch puts together.
 constexpr int PROMPT_ROWS = 128, PROMPT_KEYS = 64;
@@ -679,11 +678,12 @@ struct PromptBlock {
 // Blocks of a kv head, last ones first (they see the most keys).  false: there are fewer.
 __device__ __forceinline__ bool prompt_block(const PagedCache& c, const PagedBatch& t, int rows, int G, int index, PromptBlock& at) {
   const int lane = threadIdx.x & 63;
-  int start = 0, n = 0, blocks = 0, upto = 0, total = 0;
+  int start = 0, n = 0, length = 0, blocks = 0, upto = 0, total = 0;
   auto look = [&](int from) {
     const int i = from + lane;
     start = i < t.B ? t.starts[i] : 0;
     n = i < t.B ? t.starts[i + 1] - start : 0;
+    length = i < t.B ? paged_length(t, c.shift, i) : 0;
     n = start < 0 || start > rows || n < 0 ? 0 : min(n, rows - start);
     blocks = (int)(((int64_t)n * G + PROMPT_ROWS - 1) / PROMPT_ROWS);
     upto = paged_sums(blocks);
@@ -705,7 +705,7 @@ __device__ __forceinline__ bool prompt_block(const PagedCache& c, const PagedBat
   at.row0 = __builtin_amdgcn_readlane(start, s);
   at.n = __builtin_amdgcn_readlane(n, s);
   at.r0 = (index - before - __builtin_amdgcn_readlane(upto - blocks, s)) * PROMPT_ROWS;
-  at.length = __builtin_amdgcn_readfirstlane(paged_length(t, c.shift, at.b));
+  at.length = __builtin_amdgcn_readlane(length, s);
   return true;
 }
 // keys that the block's last row sees
@@ -760,6 +760,16 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
   const int64_t my_row = at.row0 + (valid ? token : 0);
   const int head = kvh * G + (valid ? r - token * G : 0);
 
+  // q as the products' second operand: k-step i holds elements 16 i + 8 half .. + 8 of this lane's row
+  u32x4_t qb[KS];
+  {
+    const u16* const qrow = a.q + my_row * a.ldq + head * HD;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      const uint4 x = ld16(qrow + 16 * i + 8 * half);
+      qb[i] = u32x4_t{x.x, x.y, x.z, x.w};
+    }
+  }
   // the pages of 16 keys each, 64 of these at a time; which are not there
   const int32_t* const row = t.table + (int64_t)at.b * t.ld_table;
   int pages, groups0;
@@ -781,18 +791,6 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
   };
   pages_from(t_first);
 
-  // q as the products' second operand: k-step i holds elements 16 i + 8 half .. + 8 of this lane's row
-  u32x4_t qb[KS];
-  {
-    const u16* const qrow = a.q + my_row * a.ldq + head * HD;
-#pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      const uint4 x = ld16(qrow + 16 * i + 8 * half);
-      qb[i] = u32x4_t{x.x, x.y, x.z, x.w};
-    }
-#pragma unroll
-    for (int i = 0; i < KS; ++i) asm volatile("" : "+v"(qb[i]));   // (waited for here, not behind the loads below)
-  }
   f32x16_t o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -865,9 +863,9 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
     const int piece = 4 * d + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
     vat[d] = L::TILE + (part * 32 + 4 * half + vkey) * RB + (piece ^ prompt_v_place<HD>(vkey)) * 16 + (lane & 1) * 8;
   }
-  // N tiles of 32 keys of the portion at t0
-  auto tiles = [&](auto N_, int t0, int buf) {
-    constexpr int N = decltype(N_)::value;
+  // this wave's tiles of 32 keys of the portion at t0
+  auto tiles = [&](int t0, int buf) {
+    constexpr int N = KSP == 2 ? 1 : 2;
     const int tk = t0 + part * 32;
     const unsigned char* const from = prompt_lds + buf * L::STAGE;
     f32x16_t sacc[N];
@@ -886,6 +884,7 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
 #pragma unroll
       for (int n = 0; n < N; ++n)
         sacc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, ka[i][n]), __builtin_bit_cast(bf16x8_t, qb[i]), sacc[n], 0, 0, 0);
+    __builtin_amdgcn_s_setprio(1);   // (softmax and second product ahead of the other workgroup's first one: 140 -> 136.6 us, e4m3 159 -> 151)
     // element v of tile n: key tk + 32 n + (v / 4) * 8 + half * 4 + v % 4
     const u32 lost = (u32)(gone >> ((tk - groups0) >> 4)) & (N == 2 ? 15 : 3);
     if (tk + 32 * N - 1 > pmin || lost) {   // uniform
@@ -923,9 +922,9 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
       for (int h2 = 0; h2 < 2; ++h2)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const u32 w = pack_bf2(exp2_hw(fmaf(sacc[n][8 * h2 + 2 * j], c2, nmc)), exp2_hw(fmaf(sacc[n][8 * h2 + 2 * j + 1], c2, nmc)));   // masked: 0
-          l += bf_lo(w) + bf_hi(w);
-          pw[h2][j] = w;
+          const float x0 = exp2_hw(fmaf(sacc[n][8 * h2 + 2 * j], c2, nmc)), x1 = exp2_hw(fmaf(sacc[n][8 * h2 + 2 * j + 1], c2, nmc));   // masked: 0
+          l += x0 + x1;
+          pw[h2][j] = pack_bf2(x0, x1);
         }
       // k-step h2 covers keys 16 h2 + {0..3, 8..11} + 4 half of the tile, in the order of sacc
 #pragma unroll
@@ -954,6 +953,9 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
       stage(t_first, 0);
     }
   }
+  paged_wait_loads<0>();
+#pragma unroll
+  for (int i = 0; i < KS; ++i) asm volatile("" : "+v"(qb[i]));   // (q is here with the first portion; inside the loop its wait would be one for the next portion)
   for (int t0 = t_first; t0 < t_end; t0 += PROMPT_KEYS, buf ^= 1) {
     // the portion has arrived, for all waves, and nobody reads the one before any more
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -971,15 +973,11 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
       gone = gone_now;
       groups0 = groups_now;
       const int tk = t0 + part * 32;
-      if constexpr (KSP == 2) {
-        if (tk <= pmax) tiles(std::integral_constant<int, 1>{}, t0, buf);
-      } else {
-        if (tk + 32 <= pmax) tiles(std::integral_constant<int, 2>{}, t0, buf);
-        else if (tk <= pmax) tiles(std::integral_constant<int, 1>{}, t0, buf);
-      }
+      if (tk <= pmax) tiles(t0, buf);
       gone = gone_next;
       groups0 = groups_next;
     }
+    __builtin_amdgcn_s_setprio(0);
     if constexpr (E4M3)
       if (more) expand(buf ^ 1);
   }
@@ -996,23 +994,26 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
       mine[(HD / 2 + 1) * 64] = l;
     }
     __syncthreads();
-    if (part) return;
-    // (-inf, 0, 0: no key seen; -inf, NaN, NaN: only NaN)
-    const float m1 = mine[(HD / 2) * 64], mn = fmaxf(m, m1), ref = mn == -INFINITY ? 0.0f : mn;
-    const float f0 = exp2_hw((m - ref) * c2), f1 = exp2_hw((m1 - ref) * c2);
-    l = l * f0 + mine[(HD / 2 + 1) * 64] * f1;
+    if (!part) {
+      // (-inf, 0, 0: no key seen; -inf, NaN, NaN: only NaN)
+      const float m1 = mine[(HD / 2) * 64], mn = fmaxf(m, m1), ref = mn == -INFINITY ? 0.0f : mn;
+      const float f0 = exp2_hw((m - ref) * c2), f1 = exp2_hw((m1 - ref) * c2);
+      l = l * f0 + mine[(HD / 2 + 1) * 64] * f1;
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) o[d][v] = fmaf(o[d][v], f0, mine[(d * 16 + v) * 64] * f1);
-    m = mn;
+        for (int v = 0; v < 16; ++v) o[d][v] = fmaf(o[d][v], f0, mine[(d * 16 + v) * 64] * f1);
+      m = mn;
+    }
   }
   l += __shfl_xor(l, 32, LR_WAVE);
-  if (!valid) return;
   // element v of tile d: dimension d * 32 + (v / 4) * 8 + half * 4 + v % 4
   if (!SPLIT || prompt_parts(nkeys, a.n_split) == 1) {
+    // through the wave's part of LDS, so that whole rows are stored: 16 bytes a lane, as they lie
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    u16* const yrow = a.y + my_row * a.ldy + head * HD;
+    unsigned char* const mine = prompt_lds + w4 * 32 * RB;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // (nobody reads keys and values, or the other four waves' results, any more)
+    if (part) return;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -1020,9 +1021,16 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
         uint2 w2;
         w2.x = pack_bf2(o[d][4 * g4] * inv, o[d][4 * g4 + 1] * inv);
         w2.y = pack_bf2(o[d][4 * g4 + 2] * inv, o[d][4 * g4 + 3] * inv);
-        *reinterpret_cast<uint2*>(yrow + d * 32 + g4 * 8 + half * 4) = w2;
+        *reinterpret_cast<uint2*>(mine + col * RB + ((d * 4 + g4) ^ (col & (PIECES - 1))) * 16 + half * 8) = w2;
       }
-  } else {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32 / RPL; ++i) {
+      const int k = i * RPL + lrow, rk = wr0 + k, tk = rk / G;
+      const uint4 x = *reinterpret_cast<const uint4*>(mine + k * RB + (place ^ (k & (PIECES - 1))) * 16);
+      if (rk < n_rows) st16(a.y + (at.row0 + tk) * a.ldy + (kvh * G + rk - tk * G) * HD + place * 8, x);
+    }
+  } else if (valid && !part) {
     const int64_t place_ = ((int64_t)(kvh * a.bound + index) * a.n_split + split) * PROMPT_ROWS + w4 * 32 + col;
     float* const to = a.o_part + place_ * HD;
 #pragma unroll
@@ -1034,7 +1042,7 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
   }
 }
 
-// The parts of a block's rows together: a workgroup has 16 of its 128 rows.
+// The parts of a block's rows together: a workgroup takes 1024 / HD of its 128 rows at a time, a lane four dimensions of one.
 template <int HD>
 __global__ __launch_bounds__(256) void k_paged_prompt_join(const PagedCache c, const PagedBatch t, const PagedPrompt a) {
   const int G = a.Hq / c.Hkv, kvh = blockIdx.x % c.Hkv, index = blockIdx.x / c.Hkv;
@@ -1042,37 +1050,49 @@ __global__ __launch_bounds__(256) void k_paged_prompt_join(const PagedCache c, c
   if (!prompt_block(c, t, a.rows, G, index, at)) return;
   const int parts = prompt_parts(prompt_keys(at, G), a.n_split);
   if (parts == 1) return;
-  for (int i = threadIdx.x; i < 16 * (HD / 4); i += 256) {
-    const int k = blockIdx.y * 16 + i / (HD / 4), d = i % (HD / 4) * 4, r = at.r0 + k;
-    if (r >= at.n * G) break;
-    const int64_t place = (int64_t)(kvh * a.bound + index) * a.n_split * PROMPT_ROWS + k;
-    float M = -INFINITY, L = 0.0f;
-    f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int u = 0; u < parts; u += 8) {
-      f32x4_t ov[8];
-      f32x2_t ml[8];
+  const int d = threadIdx.x % (HD / 4) * 4;
+  auto rows = [&](auto N_) __attribute__((always_inline)) {
+    constexpr int AT_ONCE = decltype(N_)::value;
+    for (int k = blockIdx.y * (1024 / HD) + threadIdx.x / (HD / 4); k < PROMPT_ROWS && at.r0 + k < at.n * G; k += gridDim.y * (1024 / HD)) {
+      const int r = at.r0 + k;
+      const int64_t place = (int64_t)(kvh * a.bound + index) * a.n_split * PROMPT_ROWS + k;
+      float M = -INFINITY, L = 0.0f;
+      f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int u = 0; u < parts; u += AT_ONCE) {
+        f32x4_t ov[AT_ONCE];
+        f32x2_t ml[AT_ONCE];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int64_t x = place + (int64_t)min(u + j, parts - 1) * PROMPT_ROWS;
-        ov[j] = *reinterpret_cast<const f32x4_t*>(a.o_part + x * HD + d);
-        ml[j] = *reinterpret_cast<const f32x2_t*>(a.ml_part + x * 2);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (u + j < parts) {
-          const float Mn = fmaxf(M, ml[j][0]), ref = Mn == -INFINITY ? 0.0f : Mn;
-          const float f0 = exp2_hw(M - ref), f1 = exp2_hw(ml[j][0] - ref);
-          L = L * f0 + ml[j][1] * f1;
-          v = v * f0 + ov[j] * f1;
-          M = Mn;
+        for (int j = 0; j < AT_ONCE; ++j) {   // (all of them on their way before the first is used; behind the last part, that one again)
+          const int64_t x = place + (int64_t)min(u + j, parts - 1) * PROMPT_ROWS;
+          ml[j] = *reinterpret_cast<const f32x2_t*>(a.ml_part + x * 2);
+          ov[j] = *reinterpret_cast<const f32x4_t*>(a.o_part + x * HD + d);
         }
+        float top = M;
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) top = fmaxf(top, ml[j][0]);
+        const float ref = top == -INFINITY ? 0.0f : top, f0 = exp2_hw(M - ref);
+        L *= f0;
+        v *= f0;
+        M = top;
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+          if (u + j < parts) {
+            const float f = exp2_hw(ml[j][0] - ref);
+            L = fmaf(f, ml[j][1], L);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = fmaf(f, ov[j][e], v[e]);
+          }
+        }
+      }
+      const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+      u32x2_t out;
+      out.x = pack_bf2(v[0] * inv, v[1] * inv);
+      out.y = pack_bf2(v[2] * inv, v[3] * inv);
+      *reinterpret_cast<u32x2_t*>(a.y + (at.row0 + r / G) * a.ldy + (kvh * G + r % G) * HD + d) = out;
     }
-    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-    u32x2_t out;
-    out.x = pack_bf2(v[0] * inv, v[1] * inv);
-    out.y = pack_bf2(v[2] * inv, v[3] * inv);
-    *reinterpret_cast<u32x2_t*>(a.y + (at.row0 + r / G) * a.ldy + (kvh * G + r % G) * HD + d) = out;
-  }
+  };
+  if (parts <= 4) rows(std::integral_constant<int, 4>{});
+  else rows(std::integral_constant<int, 16>{});
 }
 
 struct PromptPlan {
@@ -1111,7 +1131,9 @@ static int launch_prompt(const PagedCache& c, const PagedBatch& t, const PagedQu
   a.ml_part = a.o_part + (size_t)p.items * p.n_split * PROMPT_ROWS * HD;
   if (p.n_split == 1) return launch_prompt_as<HD, E4M3, 1, false>(c, t, a, (unsigned)p.items, s);
   if (const int rc = launch_prompt_as<HD, E4M3, 2, true>(c, t, a, (unsigned)(p.items * p.n_split), s)) return rc;
-  k_paged_prompt_join<HD><<<dim3((unsigned)p.items, PROMPT_ROWS / 16), dim3(256), 0, s>>>(c, t, a);
+  // (us, 16 blocks in 16 parts with 8 and 16 workgroups a block 8.2, 5.6; 128 blocks in 2 parts 7.6, 12.3)
+  const int64_t join = p.items < 64 ? PROMPT_ROWS * HD / 1024 : 1024 / p.items;
+  k_paged_prompt_join<HD><<<dim3((unsigned)p.items, (unsigned)(join < 1 ? 1 : join)), dim3(256), 0, s>>>(c, t, a);
   return lr_launch_status();
 }
 
