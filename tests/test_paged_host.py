@@ -1,4 +1,5 @@
 """The paged key-value cache without a GPU: refusals of the C entry points, the oracle's own definitions, the module's bookkeeping."""
+import copy
 import ctypes
 import math
 
@@ -19,7 +20,7 @@ def hip():
 
 
 def descs(hip, **change):
-    """(cache, batch) that are served, with some fields changed.  The addresses are never followed: nothing is launched."""
+    """(cache, batch) that are served, with some fields changed.  The addresses are nobody's: only calls that are refused are made."""
     c = dict(k=4096, v=8192, scales=12288, n_pages=10, page=16, n_kv_head=2, head_dim=128, format=1)
     b = dict(table=64, ld_table=4, lengths=128, starts=192, err=None, B=3, pages=4)
     for k, v in change.items():
@@ -27,13 +28,23 @@ def descs(hip, **change):
     return hip._PagedCache(**c), hip._PagedBatch(**b)
 
 
-def calls(hip, cache, batch, rows=5, Hq=8, ld=None, scale=0.1, x=1 << 20, rope=None, rot=128, rope_dtype=0, scratch_bytes=1 << 30):
+WRITE, READ, ATTEND = range(3)
+
+
+def calls(hip, cache, batch, which=(WRITE, READ, ATTEND), rows=5, Hq=8, ld=None, scale=0.1, x=1 << 20, rope=None, rot=128, rope_dtype=0,
+          scratch_bytes=1 << 30):
+    """What the entry points `which` return, one value where they agree."""
     lib, c, b = hip.load(), ctypes.byref(cache), ctypes.byref(batch)
     hd, hkv = max(cache.head_dim, 1), max(cache.n_kv_head, 1)
     width = ld or (Hq + 2 * hkv) * hd
-    return (lib.lr_paged_write(c, b, x, width, 1 << 21, Hq * hd, rows, Hq, rope, 64, rot, 1, rope_dtype, None),
-            lib.lr_paged_read(c, b, x, ld or hkv * hd, 1 << 21, ld or hkv * hd, rows, None),
-            lib.lr_paged_attention(c, b, x, ld or Hq * hd, 1 << 21, ld or Hq * hd, rows, Hq, scale, 1 << 22, scratch_bytes, None))
+    got = set()
+    if WRITE in which:
+        got.add(lib.lr_paged_write(c, b, x, width, 1 << 21, Hq * hd, rows, Hq, rope, 64, rot, 1, rope_dtype, None))
+    if READ in which:
+        got.add(lib.lr_paged_read(c, b, x, ld or hkv * hd, 1 << 21, ld or hkv * hd, rows, None))
+    if ATTEND in which:
+        got.add(lib.lr_paged_attention(c, b, x, ld or Hq * hd, 1 << 21, ld or Hq * hd, rows, Hq, scale, 1 << 22, scratch_bytes, None))
+    return got
 
 
 @pytest.mark.parametrize("change,code", [
@@ -48,10 +59,8 @@ def calls(hip, cache, batch, rows=5, Hq=8, ld=None, scale=0.1, x=1 << 20, rope=N
     (dict(starts=None), E_SHAPE),      # one row per sequence: 3, not 5
 ])
 def test_descriptors_are_checked_by_every_entry_point(hip, change, code):
-    got = calls(hip, *descs(hip, **change))
-    if change == dict(n_kv_head=3):    # 8 q heads on 3: a read has no q heads
-        got = got[0], got[2]
-    assert set(got) == {code}
+    which = (WRITE, ATTEND) if change == dict(n_kv_head=3) else (WRITE, READ, ATTEND)    # 8 q heads on 3: a read has no q heads
+    assert calls(hip, *descs(hip, **change), which) == {code}
     cache, batch = descs(hip, **change)
     if change not in (dict(starts=None),):
         assert hip.load().lr_paged_attention_scratch_bytes(ctypes.byref(cache), ctypes.byref(batch), 5, 8) == 0
@@ -64,18 +73,19 @@ def test_arguments_are_checked(hip):
         assert lib.lr_paged_write(n, ctypes.byref(d[1]), 16, 8, 16, 8, 1, 8, None, 0, 0, 0, 0, None) == E_NULL
         assert lib.lr_paged_read(ctypes.byref(d[0]), n, 16, 8, 16, 8, 1, None) == E_NULL
         assert lib.lr_paged_attention(n, n, 16, 8, 16, 8, 1, 8, 1.0, 16, 1 << 30, None) == E_NULL
-    assert set(calls(hip, *d, rows=0)) == {E_SHAPE}
-    assert set(calls(hip, *d, x=None)) == {E_NULL}
-    assert set(calls(hip, *d, x=(1 << 20) + 8)) == {E_ALIGN}
-    assert calls(hip, *d, ld=255)[1] == E_SHAPE and set(calls(hip, *d, ld=12 * 128 + 4)) == {E_ALIGN}
-    assert calls(hip, *d, ld=8)[::2] == (E_SHAPE, E_SHAPE)
-    assert calls(hip, *d, Hq=7)[::2] == (E_SHAPE, E_SHAPE)
+    heads = WRITE, ATTEND
+    assert calls(hip, *d, rows=0) == {E_SHAPE}
+    assert calls(hip, *d, x=None) == {E_NULL}
+    assert calls(hip, *d, x=(1 << 20) + 8) == {E_ALIGN}
+    assert calls(hip, *d, ld=248) == {E_SHAPE} and calls(hip, *d, ld=12 * 128 + 4) == {E_ALIGN}
+    assert calls(hip, *d, heads, ld=8) == {E_SHAPE}
+    assert calls(hip, *d, heads, Hq=7) == {E_SHAPE}
     for scale in (0.0, -1.0, math.nan, math.inf):
-        assert calls(hip, *d, scale=scale)[2] == E_SHAPE
-    assert calls(hip, *d, scratch_bytes=0)[2] == E_SHAPE
-    assert calls(hip, *d, rope=64, rot=144)[0] == E_SHAPE and calls(hip, *d, rope=64, rot=0)[0] == E_SHAPE
-    assert calls(hip, *d, rope=64, rot=24)[0] == E_UNSUPPORTED and calls(hip, *d, rope=64, rope_dtype=2)[0] == E_UNSUPPORTED
-    assert calls(hip, *d, rope=68)[0] == E_ALIGN
+        assert calls(hip, *d, (ATTEND,), scale=scale) == {E_SHAPE}
+    assert calls(hip, *d, (ATTEND,), scratch_bytes=0) == {E_SHAPE}
+    assert calls(hip, *d, (WRITE,), rope=64, rot=144) == {E_SHAPE} and calls(hip, *d, (WRITE,), rope=64, rot=0) == {E_SHAPE}
+    assert calls(hip, *d, (WRITE,), rope=64, rot=24) == {E_UNSUPPORTED} and calls(hip, *d, (WRITE,), rope=64, rope_dtype=2) == {E_UNSUPPORTED}
+    assert calls(hip, *d, (WRITE,), rope=68) == {E_ALIGN}
 
 
 def test_scratch_grows_with_what_is_served(hip):
@@ -92,7 +102,7 @@ def test_module_bookkeeping():
     from gpt_fast.utils import PagedKVCache
 
     c = PagedKVCache(5, 32, 2, 64)
-    assert c.scales is None and c.shape == (2, 32, 64) and c.k_pages.dtype == torch.bfloat16
+    assert c.scales is None and c.shape == (2, 32, 64, torch.bfloat16)
     c = PagedKVCache(5, 32, 2, 64, torch.float8_e4m3fn)
     assert tuple(c.scales.shape) == (5, 2, 2, 32) and c.scales.dtype == torch.uint8
     c.to(torch.float32)          # a model's type is not its cache's
@@ -100,6 +110,8 @@ def test_module_bookkeeping():
     assert set(c.state_dict()) == {"k_pages", "v_pages", "scales"}
     with pytest.raises(AssertionError):
         PagedKVCache(5, 32, 2, 64, torch.float32)
+    twin = copy.deepcopy(c)
+    assert twin.k_pages.data_ptr() != c.k_pages.data_ptr() and twin.shape == c.shape
     t = torch.zeros(2, 3, dtype=torch.int32)
     with pytest.raises(AssertionError, match="rows"):
         c.batch(t, t[:, 0], 4, starts=torch.zeros(3, dtype=torch.int32))
