@@ -1096,7 +1096,7 @@ __global__ __launch_bounds__(256) void k_paged_prompt_join(const PagedCache c, c
 }
 
 struct PromptPlan {
-  int bound, n_split;
+  int bound, n_split, waves;   // waves: four or eight of a workgroup
   int64_t items;
   size_t bytes;   // of parts that any number of rows could need
 };
@@ -1115,6 +1115,9 @@ static PromptPlan prompt_plan(const PagedCache& c, const PagedBatch& t, int hd, 
   const int64_t portions = (((int64_t)t.pages << c.shift) + PROMPT_KEYS - 1) / PROMPT_KEYS;
   if (n < 1 || portions * (n - 1) <= 8 * n) n = 1;
   p.n_split = (int)n;
+  // eight waves where they would be the CU's only ones and have something to share (us, four / eight: 700 tokens of 12 heads of 64 14.5 / 12.7,
+  // 300 of the 8B model 12.0 / 12.2, 100 of 32 heads of 64 6.8 / 7.3)
+  p.waves = n > 1 || (p.items <= cus && portions >= 8) ? 8 : 4;
   p.bytes = most > 1 ? (size_t)cus * PROMPT_ROWS * (hd + 2) * 4 : 0;
   return p;
 }
@@ -1133,7 +1136,8 @@ static int launch_prompt(const PagedCache& c, const PagedBatch& t, const PagedQu
   if (p.items * p.n_split > (1 << 24)) return LR_E_UNSUPPORTED;   // (workgroups of a grid)
   PagedPrompt a = {q.q, q.ldq, q.y, q.ldy, q.rows, q.Hq, p.n_split, p.bound, q.scale, (float*)scratch, nullptr};
   a.ml_part = a.o_part + (size_t)p.items * p.n_split * PROMPT_ROWS * HD;
-  if (p.n_split == 1) return launch_prompt_as<HD, E4M3, 1, false>(c, t, a, (unsigned)p.items, s);
+  if (p.n_split == 1)
+    return p.waves == 8 ? launch_prompt_as<HD, E4M3, 2, false>(c, t, a, (unsigned)p.items, s) : launch_prompt_as<HD, E4M3, 1, false>(c, t, a, (unsigned)p.items, s);
   if (const int rc = launch_prompt_as<HD, E4M3, 2, true>(c, t, a, (unsigned)(p.items * p.n_split), s)) return rc;
   // (us, 16 blocks in 16 parts with 8 and 16 workgroups a block 8.2, 5.6; 128 blocks in 2 parts 7.6, 12.3)
   const int64_t join = p.items < 64 ? PROMPT_ROWS * HD / 1024 : 1024 / p.items;
