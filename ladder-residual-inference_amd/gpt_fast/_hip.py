@@ -1398,8 +1398,10 @@ def paged_cache_desc(k, v, scales=None) -> _PagedCache:
     if e4m3:
         assert tuple(scales.shape) == (n, heads, 2, page) and scales.is_contiguous() and scales.device == k.device
     assert v.device == k.device
-    return _PagedCache(_dev(k, dtype), _dev(v, dtype), _dev(scales, torch.uint8) if e4m3 else None, n, page, heads, hd,
-                       CACHE_E4M3 if e4m3 else CACHE_BF16)
+    d = _PagedCache(_dev(k, dtype), _dev(v, dtype), _dev(scales, torch.uint8) if e4m3 else None, n, page, heads, hd,
+                    CACHE_E4M3 if e4m3 else CACHE_BF16)
+    d.at, d.device = ctypes.addressof(d), k.device.index     # (looked up once: a call's checks are most of its host time)
+    return d
 
 
 def paged_batch_desc(table, lengths, starts=None) -> _PagedBatch:
@@ -1410,16 +1412,18 @@ def paged_batch_desc(table, lengths, starts=None) -> _PagedBatch:
     if starts is not None:
         assert tuple(starts.shape) == (B + 1,) and starts.is_contiguous() and starts.device == table.device
     i = torch.int32
-    return _PagedBatch(_dev(table, i), max(table.stride(0), pages), _dev(lengths, i), None if starts is None else _dev(starts, i),
-                       device_error_word(table.device).data_ptr(), B, pages)
+    d = _PagedBatch(_dev(table, i), max(table.stride(0), pages), _dev(lengths, i), None if starts is None else _dev(starts, i),
+                    device_error_word(table.device).data_ptr(), B, pages)
+    d.at = ctypes.addressof(d)
+    return d
 
 
 def _paged_rows(t, width, device):
     """(address, row stride, rows) of a [rows, width] bf16 matrix with dense rows."""
     rows, cols = t.shape
     ld, unit = t.stride()
-    if t.dtype != torch.bfloat16 or cols != width or unit != 1 or t.device != device:
-        raise ValueError(f"expected [rows, {width}] bfloat16 with dense rows on {device}, got {tuple(t.shape)} {t.dtype} "
+    if t.dtype is not torch.bfloat16 or cols != width or unit != 1 or t.get_device() != device:
+        raise ValueError(f"expected [rows, {width}] bfloat16 with dense rows on cuda:{device}, got {tuple(t.shape)} {t.dtype} "
                          f"with strides {t.stride()} on {t.device}")
     return t.data_ptr(), (ld if rows > 1 else cols), rows
 
@@ -1427,53 +1431,59 @@ def _paged_rows(t, width, device):
 def _paged_stream(device) -> int:
     """The current stream of the device that the cache is on, which has to be the current one.  (torch.cuda.current_stream() builds an object
     each time: 2.6 us of a call's 9, this 0.2.)"""
-    if torch._C._cuda_getDevice() != device.index:
-        raise ValueError(f"the cache is on {device}, the current device is cuda:{torch.cuda.current_device()}")
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    if torch._C._cuda_getDevice() != device:
+        raise ValueError(f"the cache is on cuda:{device}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
-def paged_write(cache, batch, qkv, q, n_head, device, rope=None, interleaved=True):
+def paged_write(cache, batch, qkv, q, n_head, rope=None, interleaved=True):
     """lr_paged_write: qkv [rows, (n_head + 2 kv heads) head_dim], q [rows, n_head head_dim]; rope [positions, rot / 2, 2] bf16 or fp32."""
-    hd = cache.head_dim
+    hd, device = cache.head_dim, cache.device
     x, ldx, rows = _paged_rows(qkv, (n_head + 2 * cache.n_kv_head) * hd, device)
     o, ldo, n = _paged_rows(q, n_head * hd, device)
     if n != rows:
         raise ValueError(f"{rows} rows of qkv, {n} of q")
-    r, length, rot, f32 = None, 0, 0, 0
+    r, length, rot, kind = None, 0, 0, 0
     if rope is not None:
-        length, rot = rope.shape[0], 2 * rope.shape[1]
-        if rope.dim() != 3 or rope.shape[2] != 2 or not rope.is_contiguous() or rope.device != device or \
-                rope.dtype not in (torch.bfloat16, torch.float32):
-            raise ValueError(f"rope is dense [positions, rot / 2, 2], bfloat16 or float32, on {device}")
-        r, f32 = rope.data_ptr(), int(rope.dtype == torch.float32)
-    _check(load().lr_paged_write(ctypes.byref(cache), ctypes.byref(batch), x, ldx, o, ldo, rows, n_head, r, length, rot, int(interleaved), f32,
-                                 _paged_stream(device)), "lr_paged_write")
+        length, rot, two = rope.shape
+        kind = 0 if rope.dtype is torch.bfloat16 else 1 if rope.dtype is torch.float32 else -1
+        if two != 2 or kind < 0 or not rope.is_contiguous() or rope.get_device() != device:
+            raise ValueError(f"rope is dense [positions, rot / 2, 2], bfloat16 or float32, on cuda:{device}")
+        r, rot = rope.data_ptr(), 2 * rot
+    rc = _lib.lr_paged_write(cache.at, batch.at, x, ldx, o, ldo, rows, n_head, r, length, rot, interleaved, kind, _paged_stream(device))
+    if rc:
+        _check(rc, "lr_paged_write")
     return q
 
 
-def paged_read(cache, batch, k, v, device):
+def paged_read(cache, batch, k, v):
     """lr_paged_read: k, v [rows, kv heads * head_dim]."""
-    a, lda, rows = _paged_rows(k, cache.n_kv_head * cache.head_dim, device)
-    b, ldb, n = _paged_rows(v, cache.n_kv_head * cache.head_dim, device)
+    width, device = cache.n_kv_head * cache.head_dim, cache.device
+    a, lda, rows = _paged_rows(k, width, device)
+    b, ldb, n = _paged_rows(v, width, device)
     if n != rows:
         raise ValueError(f"{rows} rows of k, {n} of v")
-    _check(load().lr_paged_read(ctypes.byref(cache), ctypes.byref(batch), a, lda, b, ldb, rows, _paged_stream(device)), "lr_paged_read")
+    rc = _lib.lr_paged_read(cache.at, batch.at, a, lda, b, ldb, rows, _paged_stream(device))
+    if rc:
+        _check(rc, "lr_paged_read")
     return k, v
 
 
 def paged_attention_scratch_bytes(cache, batch, rows, n_head) -> int:
-    return int(load().lr_paged_attention_scratch_bytes(ctypes.byref(cache), ctypes.byref(batch), rows, n_head))
+    return int(load().lr_paged_attention_scratch_bytes(cache.at, batch.at, rows, n_head))
 
 
-def paged_attention(cache, batch, q, y, n_head, device, scratch, scale=None):
+def paged_attention(cache, batch, q, y, n_head, scratch, scale=None):
     """lr_paged_attention: q, y [rows, n_head * head_dim]; scratch uint8, zero before the first call."""
-    x, ldx, rows = _paged_rows(q, n_head * cache.head_dim, device)
-    o, ldo, n = _paged_rows(y, n_head * cache.head_dim, device)
+    hd, device = cache.head_dim, cache.device
+    x, ldx, rows = _paged_rows(q, n_head * hd, device)
+    o, ldo, n = _paged_rows(y, n_head * hd, device)
     if n != rows:
         raise ValueError(f"{rows} rows of q, {n} of y")
-    _check(load().lr_paged_attention(ctypes.byref(cache), ctypes.byref(batch), x, ldx, o, ldo, rows, n_head,
-                                     cache.head_dim ** -0.5 if scale is None else scale, scratch.data_ptr(), scratch.numel(),
-                                     _paged_stream(device)), "lr_paged_attention")
+    rc = _lib.lr_paged_attention(cache.at, batch.at, x, ldx, o, ldo, rows, n_head, hd ** -0.5 if scale is None else scale, scratch.data_ptr(),
+                                 scratch.numel(), _paged_stream(device))
+    if rc:
+        _check(rc, "lr_paged_attention")
     return y
 
 

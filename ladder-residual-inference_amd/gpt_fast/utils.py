@@ -65,7 +65,8 @@ class PagedBatch:
 
     def __init__(self, cache: "PagedKVCache", table: Tensor, lengths: Tensor, n_head: int, starts: Optional[Tensor], rows: int):
         self.table, self.lengths, self.starts, self.n_head, self.rows = table, lengths, starts, n_head, rows
-        self.shape, self.device = cache.shape, table.device
+        self.shape = cache.shape
+        assert table.device == cache.k_pages.device, "the tables are where the pages are"
         self.desc = _hip.paged_batch_desc(table, lengths, starts)
         need = _hip.paged_attention_scratch_bytes(cache.desc(), self.desc, rows, n_head)
         if need == 0:
@@ -112,13 +113,13 @@ class PagedKVCache(nn.Module):
 
     @property
     def shape(self):
-        """(kv heads, page, head_dim, type): a batch serves caches of the same."""
-        return (*self.k_pages.shape[1:], self.k_pages.dtype)
+        """(kv heads, page, head_dim, type, device): a batch serves caches of the same."""
+        return (*self.k_pages.shape[1:], self.k_pages.dtype, self.k_pages.device)
 
     def desc(self):
         if self._desc is None:
             self._desc = _hip.paged_cache_desc(self.k_pages, self.v_pages, self.scales)
-            self._device, self._shape = self.k_pages.device, self.shape
+            self._shape = self.shape
         return self._desc
 
     def _apply(self, fn, recurse=True):
@@ -137,24 +138,23 @@ class PagedKVCache(nn.Module):
 
     def _check(self, batch: PagedBatch, rows: int):
         desc = self._desc or self.desc()
-        if batch.shape != self._shape or rows > batch.rows or batch.device != self._device:
-            raise ValueError(f"a batch for up to {batch.rows} rows and pages {batch.shape} on {batch.device}: got {rows} rows, pages {self._shape} "
-                             f"on {self._device}")
+        if batch.shape != self._shape or rows > batch.rows:
+            raise ValueError(f"a batch for up to {batch.rows} rows and pages {batch.shape}: got {rows} rows, pages {self._shape}")
         return desc
 
     def write(self, batch: PagedBatch, qkv: Tensor, q: Tensor, rope: Optional[Tensor] = None, interleaved: bool = True) -> Tensor:
         """qkv [rows, (n_head + 2 kv heads) head_dim] fresh from the fused projection: q and k rotated by rope [positions, rot / 2, 2]
         (precompute_freqs_cis's table, or fp32; pairs of neighbours, or of the two halves of the first rot dimensions), q to `q` (which may
         be qkv's own columns), k and v into the pages."""
-        return _hip.paged_write(self._check(batch, qkv.shape[0]), batch.desc, qkv, q, batch.n_head, self._device, rope, interleaved)
+        return _hip.paged_write(self._check(batch, qkv.shape[0]), batch.desc, qkv, q, batch.n_head, rope, interleaved)
 
     def read(self, batch: PagedBatch, k: Tensor, v: Tensor):
         """The call's tokens back, [rows, kv heads * head_dim] bf16."""
-        return _hip.paged_read(self._check(batch, k.shape[0]), batch.desc, k, v, self._device)
+        return _hip.paged_read(self._check(batch, k.shape[0]), batch.desc, k, v)
 
     def attend(self, batch: PagedBatch, q: Tensor, y: Tensor, scale: Optional[float] = None) -> Tensor:
         """y [rows, n_head * head_dim] = attention of the rotated q's rows, each on its sequence's keys up to its own position."""
-        return _hip.paged_attention(self._check(batch, q.shape[0]), batch.desc, q, y, batch.n_head, self._device, batch.scratch, scale)
+        return _hip.paged_attention(self._check(batch, q.shape[0]), batch.desc, q, y, batch.n_head, batch.scratch, scale)
 
 
 class RMSNorm(nn.Module):

@@ -102,7 +102,7 @@ def test_module_bookkeeping():
     from gpt_fast.utils import PagedKVCache
 
     c = PagedKVCache(5, 32, 2, 64)
-    assert c.scales is None and c.shape == (2, 32, 64, torch.bfloat16)
+    assert c.scales is None and c.shape == (2, 32, 64, torch.bfloat16, torch.device("cpu"))
     c = PagedKVCache(5, 32, 2, 64, torch.float8_e4m3fn)
     assert tuple(c.scales.shape) == (5, 2, 2, 32) and c.scales.dtype == torch.uint8
     c.to(torch.float32)          # a model's type is not its cache's
