@@ -760,6 +760,26 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
   const int64_t my_row = at.row0 + (valid ? token : 0);
   const int head = kvh * G + (valid ? r - token * G : 0);
 
+  // the pages of 16 keys each, 64 of these at a time; which are not there
+  const int32_t* const row = t.table + (int64_t)at.b * t.ld_table;
+  int pages, groups0;
+  unsigned long long gone;
+  auto ask_pages = [&](int key0) {
+    groups0 = key0;
+    const int key = key0 + 16 * lane;
+    pages = key < t_end ? row[key >> c.shift] : 0;
+  };
+  auto check_pages = [&]() {
+    const bool bad = (u32)pages >= (u32)c.n_pages;
+    if (bad && t.err) *t.err = LR_DEV_PAGE_RANGE;
+    pages = bad || groups0 + 16 * lane >= t_end ? -1 : pages;
+    gone = __ballot(bad);
+  };
+  auto pages_from = [&](int key0) {
+    ask_pages(key0);
+    check_pages();
+  };
+  ask_pages(t_first);
   // q as the products' second operand: k-step i holds elements 16 i + 8 half .. + 8 of this lane's row
   u32x4_t qb[KS];
   {
@@ -770,27 +790,7 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
       qb[i] = u32x4_t{x.x, x.y, x.z, x.w};
     }
   }
-  // the pages of 16 keys each, 64 of these at a time; which are not there
-  const int32_t* const row = t.table + (int64_t)at.b * t.ld_table;
-  int pages, groups0;
-  unsigned long long gone;
-  auto pages_from = [&](int key0) {
-    groups0 = key0;
-    const int key = key0 + 16 * lane;
-    pages = -1;
-    bool bad = false;
-    if (key < t_end) {
-      pages = row[key >> c.shift];
-      bad = (u32)pages >= (u32)c.n_pages;
-      if (bad) {
-        pages = -1;
-        if (t.err) *t.err = LR_DEV_PAGE_RANGE;
-      }
-    }
-    gone = __ballot(bad);
-  };
-  pages_from(t_first);
-
+  check_pages();   // (asked for ahead of q: what is asked for comes in its order)
   f32x16_t o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -878,7 +878,8 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
     for (int i = 0; i < KS; ++i)
 #pragma unroll
       for (int n = 0; n < N; ++n) ka[i][n] = *reinterpret_cast<const u32x4_t*>(from + (kat ^ (32 * i)) + n * 32 * RB);
-    __builtin_amdgcn_sched_barrier(0);
+    // (all of them on their way before the first product: 136 -> 134.5 us; e4m3 has no registers for that)
+    if constexpr (!E4M3) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < KS; ++i)
 #pragma unroll
@@ -923,7 +924,7 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float x0 = exp2_hw(fmaf(sacc[n][8 * h2 + 2 * j], c2, nmc)), x1 = exp2_hw(fmaf(sacc[n][8 * h2 + 2 * j + 1], c2, nmc));   // masked: 0
-          l += x0 + x1;
+          l += x0 + x1;   // (v_dot2_f32_bf16 on the rounded pair would be one instruction: the compiler reads the vector's first element for all four)
           pw[h2][j] = pack_bf2(x0, x1);
         }
       // k-step h2 covers keys 16 h2 + {0..3, 8..11} + 4 half of the tile, in the order of sacc
