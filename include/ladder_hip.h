@@ -801,7 +801,7 @@ int lr_linear_multi_route(const lr_projection_t* projections, int n_projections,
  * A batch is B sequences: table [B, pages] (row stride ld_table) names their pages in order, lengths [B] how many tokens they have,
  * the call's own among them.  starts [B + 1], ascending from 0: the call's rows starts[b] .. starts[b + 1] - 1 are the last tokens of
  * sequence b, in order, i.e. row r is at position lengths[b] - starts[b + 1] + r; none for a sequence that takes no part; rows from
- * starts[B] on are left as they were.  NULL: one row per sequence (rows == B), its last token; a sequence of length 0 is an empty place.
+ * starts[B] on are left as they were, and a call of fewer rows does those.  NULL: one row per sequence (rows == B), its last token; a sequence of length 0 is an empty place.
  * All int32, read on the device (a captured call may be replayed after they have changed there).  Entries of the table behind a
  * sequence's length are not read.  Several sequences may share a page that none of them writes.
  * Conditions only the device can see set *err (may be NULL): a position outside the table's pages or the angles LR_DEV_POS_RANGE, a page
@@ -821,7 +821,7 @@ typedef struct lr_paged_batch {
 } lr_paged_batch_t;
 
 /* A call's rows [q | k | v] (qkv [rows, (Hq + 2 n_kv_head) head_dim], row stride ldqkv) into the cache: q and k rotated, q to
- * q [rows, Hq head_dim] (row stride ldq; where it lies in qkv or elsewhere, not across), k and v to their places.  rope [rope_len, rot / 2, 2]
+ * q [rows, Hq head_dim] (row stride ldq; where it lies in qkv or elsewhere: LR_E_SHAPE across), k and v to their places.  rope [rope_len, rot / 2, 2]
  * holds (cos, sin) per position, bf16 or fp32 (rope_dtype LR_BF16 or LR_F32): the first rot dimensions of a head are turned as pairs
  * (2i, 2i + 1) where interleaved != 0, (i, i + rot / 2) else; products and sums in fp32, each rounded by itself, as lr_rope_kv_write.
  * rot % 16 == 0; rope NULL: nothing is turned.  An e4m3 row is rounded from the fp32 values.  A row whose position or page is out of range is
@@ -829,16 +829,19 @@ typedef struct lr_paged_batch {
 int lr_paged_write(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, const void* qkv, int64_t ldqkv, void* q, int64_t ldq,
                    int rows, int Hq, const void* rope, int rope_len, int rot, int interleaved, int rope_dtype, lr_stream_t stream);
 
-/* The call's tokens back from the cache: k, v [rows, n_kv_head head_dim] bf16 (row strides ldk, ldv).  With starts the running sum of
+/* The call's tokens back from the cache: k, v [rows, n_kv_head head_dim] bf16 (row strides ldk, ldv), apart from each other.  With starts the running sum of
  * lengths these are whole sequences.  A row whose position or page is out of range is left as it was. */
 int lr_paged_read(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, void* k, int64_t ldk, void* v, int64_t ldv, int rows,
                   lr_stream_t stream);
 
 /* y[r, h] = softmax_j( q[r, h] . K[j, h / G] * scale ) V[j, h / G] over the keys j of row r's sequence up to its own position, G =
- * Hq / n_kv_head; q, y [rows, Hq head_dim] (row strides ldq, ldy; y is not q).  The cache holds the call's tokens already.  A row
- * that sees no key is zeros; keys of a page out of range, and those behind the table's pages, count as not there.  Scores, softmax and
- * sums in fp32, one rounding of y.  scratch: lr_paged_attention_scratch_bytes() (0: sizes that are refused), zero before the first
- * call, not shared by calls that may overlap; a size that served a batch serves one with fewer rows or shorter sequences. */
+ * Hq / n_kv_head; q, y [rows, Hq head_dim] (row strides ldq, ldy) with no memory in common.  The cache holds the call's tokens already.
+ * A row that sees no key is zeros; keys of a page out of range, and those behind the table's pages, count as not there; what keys that a
+ * row does not see hold, NaN too, does not reach it.  Scores, softmax and sums in fp32; a weight enters the matrix cores as two bf16
+ * numbers where starts is NULL, else as one; one rounding of y.  scale: positive, up to 2^64.
+ * scratch: lr_paged_attention_scratch_bytes() (0: sizes that are refused), zero before the first call and kept for calls with the same
+ * cache but for its addresses and n_pages, the same B, pages, Hq and starts or none (rows no more than those it was sized for), one
+ * after the other: calls that may overlap have their own. */
 size_t lr_paged_attention_scratch_bytes(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, int rows, int Hq);
 int lr_paged_attention(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, const void* q, int64_t ldq, void* y, int64_t ldy,
                        int rows, int Hq, float scale, void* scratch, size_t scratch_bytes, lr_stream_t stream);

@@ -2,6 +2,7 @@
 #include "paged_common.h"
 
 #include <atomic>
+#include <cfloat>
 #include <type_traits>
 
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
@@ -179,7 +180,7 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
   unsigned char* const mine = paged_lds + wave * T::WAVE;
   const int lrow = lane / T::PIECES, place = lane % T::PIECES;
   const float c2 = a.scale * 1.4426950408889634f;   // e^(x scale) = 2^(x c2)
-  const float tau = PAGED_TAU2 / c2;
+  const float tau = fminf(PAGED_TAU2 / c2, FLT_MAX);   // (-inf + tau stays -inf)
 
   // this worker's tiles from .. to of the n_tiles of a sequence, the first of which is at `first` of the line, behind the sequence's own cost
   struct Segment {
@@ -616,7 +617,7 @@ struct DecodePlan {
   size_t o_bytes, ml_bytes, ticket_bytes;
 };
 // Workers of a kv head (a group of up to 16 of its q heads): as many as the chip holds at once, no more than the table's pages could give
-// four tiles each.
+// four tiles each, one for each of their waves.
 template <int HD, bool E4M3>
 static DecodePlan decode_plan(const PagedCache& c, const PagedBatch& t, int Hq) {
   DecodePlan p;
@@ -673,18 +674,19 @@ struct PagedPrompt {
 
 // Which rows a block has.
 struct PromptBlock {
-  int b, row0, n, length, r0;     // sequence, its first row of the call and their number, its keys; the block's first row of the kv head's
+  int b, row0, n, ahead, r0;     // sequence, its first row of the call and their number, its tokens ahead of them; the block's first row of the kv head's
 };
 // Blocks of a kv head, last ones first (they see the most keys).  false: there are fewer.
 __device__ __forceinline__ bool prompt_block(const PagedCache& c, const PagedBatch& t, int rows, int G, int index, PromptBlock& at) {
   const int lane = threadIdx.x & 63;
-  int start = 0, n = 0, length = 0, blocks = 0, upto = 0, total = 0;
+  int start = 0, n = 0, ahead = 0, blocks = 0, upto = 0, total = 0;
   auto look = [&](int from) {
     const int i = from + lane;
     start = i < t.B ? t.starts[i] : 0;
     n = i < t.B ? t.starts[i + 1] - start : 0;
-    length = i < t.B ? paged_length(t, c.shift, i) : 0;
-    n = start < 0 || start > rows || n < 0 ? 0 : min(n, rows - start);
+    n = start < 0 || start > rows || n < 0 ? 0 : n;
+    ahead = (i < t.B ? paged_length(t, c.shift, i) : 0) - n;
+    n = min(n, rows - start);   // (a call may have fewer rows than starts says)
     blocks = (int)(((int64_t)n * G + PROMPT_ROWS - 1) / PROMPT_ROWS);
     upto = paged_sums(blocks);
     return __builtin_amdgcn_readlane(upto, 63);
@@ -705,13 +707,13 @@ __device__ __forceinline__ bool prompt_block(const PagedCache& c, const PagedBat
   at.row0 = __builtin_amdgcn_readlane(start, s);
   at.n = __builtin_amdgcn_readlane(n, s);
   at.r0 = (index - before - __builtin_amdgcn_readlane(upto - blocks, s)) * PROMPT_ROWS;
-  at.length = __builtin_amdgcn_readlane(length, s);
-  return true;
+  at.ahead = __builtin_amdgcn_readlane(ahead, s);
+  return at.r0 >= 0 && at.r0 < at.n * G;   // (starts that do not ascend name more blocks than 32 bits count)
 }
 // keys that the block's last row sees
 __device__ __forceinline__ int prompt_keys(const PromptBlock& at, int G) {
   const int last = min(at.r0 + PROMPT_ROWS, at.n * G) - 1;
-  return max(0, at.length - at.n + last / G + 1);
+  return max(0, at.ahead + last / G + 1);
 }
 // and into how many parts they are cut
 __device__ __forceinline__ int prompt_parts(int keys, int n_split) { return max(1, min(n_split, (keys + PROMPT_SPLIT_KEYS - 1) / PROMPT_SPLIT_KEYS)); }
@@ -752,11 +754,11 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
     t_end = min(nkeys, (int)((int64_t)portions * (split + 1) / parts) * PROMPT_KEYS);
   }
   // this lane's row, the last key that it sees, and the smallest and largest of the wave's
-  const int n_rows = at.n * G, r = at.r0 + w4 * 32 + col, token = r / G, ahead = at.length - at.n;
+  const int n_rows = at.n * G, r = at.r0 + w4 * 32 + col, token = r / G;
   const bool valid = r < n_rows;
-  const int p = valid ? ahead + token : -1;
+  const int p = valid ? at.ahead + token : -1;
   const int wr0 = at.r0 + w4 * 32;
-  const int pmin = __builtin_amdgcn_readfirstlane(ahead + wr0 / G), pmax = __builtin_amdgcn_readfirstlane(wr0 < n_rows ? ahead + (min(wr0 + 32, n_rows) - 1) / G : -1);
+  const int pmin = __builtin_amdgcn_readfirstlane(at.ahead + wr0 / G), pmax = __builtin_amdgcn_readfirstlane(wr0 < n_rows ? at.ahead + (min(wr0 + 32, n_rows) - 1) / G : -1);
   const int64_t my_row = at.row0 + (valid ? token : 0);
   const int head = kvh * G + (valid ? r - token * G : 0);
 
@@ -797,7 +799,7 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
   float m = -INFINITY, l = 0.0f;   // m: reference point in raw scores; l: this lane's half of the row's sum
-  const float c2 = a.scale * 1.4426950408889634f, tau = PAGED_TAU2 / c2;
+  const float c2 = a.scale * 1.4426950408889634f, tau = fminf(PAGED_TAU2 / c2, FLT_MAX);
 
   // ---- loads of a portion
   constexpr int RPL = 1024 / RB, LOADS = PROMPT_KEYS / RPL / NW;   // bf16: rows per load instruction; a wave's loads of K or V
@@ -899,7 +901,7 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
     }
     float top = sacc[0][0];
 #pragma unroll
-    for (int v = 1; v < 16 * N; ++v) top = __builtin_amdgcn_fmed3f(top, sacc[v / 16][v % 16], INFINITY);   // (the larger; see k_attn_prefill_mfma)
+    for (int v = 1; v < 16 * N; ++v) top = __builtin_amdgcn_fmed3f(top, sacc[v / 16][v % 16], INFINITY);   // (the larger of two: one instruction, where fmaxf takes a second that makes NaN quiet)
     {
       const u32 u = __float_as_uint(top);
       const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
@@ -981,6 +983,80 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
     __builtin_amdgcn_s_setprio(0);
     if constexpr (E4M3)
       if (more) expand(buf ^ 1);
+  }
+  // The products take a tile's values for all rows: one that is not finite reached also those that do not see its key, as 0 * v.  Rare, and
+  // not worth a look at every value: a wave that ends with something that is not finite, and has such a value among the keys that
+  // not all of its rows see, does its rows again, key by key.
+  {
+    float none = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) none = fmaf(o[d][v], 0.0f, none);
+    if (__any(none != none)) {
+      auto my_key = [&](int key) { return key >= t_first && key < t_end && (KSP == 1 || ((key - t_first) >> 5 & 1) == part); };
+      auto page_of = [&](int key) {
+        const int page = row[key >> c.shift];
+        return (u32)page < (u32)c.n_pages ? page : -1;
+      };
+      // elements d .. d + 3 of a key's row
+      auto four = [&](bool value, int page, int key, int d) {
+        const int slot = key & ((1 << c.shift) - 1);
+        const u8* const from = (value ? c.v : c.k) + paged_offset<HD * (E4M3 ? 1 : 2)>(c, page, kvh) + (slot * HD + d) * (E4M3 ? 1 : 2);
+        u32x2_t x;
+        if constexpr (E4M3) {
+          const u32 u = *reinterpret_cast<const u32*>(from);
+          const float s = paged_scale(c.scales[paged_scales(c, page, kvh) + ((int)value << c.shift) + slot]);
+          x.x = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u, s, false));
+          x.y = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u, s, true));
+        } else {
+          x = *reinterpret_cast<const u32x2_t*>(from);
+        }
+        return f32x4_t{bf_lo(x.x), bf_hi(x.x), bf_lo(x.y), bf_hi(x.y)};
+      };
+      bool some = false;
+#pragma unroll 1
+      for (int key = max(0, pmin + 1); key < pmax + PROMPT_KEYS; ++key) {   // (those of its last portion that none of them sees, too)
+        const int page = my_key(key) ? page_of(key) : -1;
+        if (page < 0) continue;
+        const f32x4_t v = four(true, page, key, lane * 4 % HD);
+        some |= !(fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY);
+      }
+      if (__any(some)) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
+        const float nmc = m == -INFINITY ? 0.0f : -m * c2;
+#pragma unroll 1
+        for (int key = t_first; key < t_end && key <= pmax; ++key) {
+          const int page = my_key(key) ? page_of(key) : -1;
+          if (page < 0) continue;
+          float s = 0.0f;
+#pragma unroll
+          for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+              const f32x4_t k4 = four(false, page, key, 16 * i + 8 * half + j);
+              const u32 q0 = qb[i][j / 2], q1 = qb[i][j / 2 + 1];
+              s = fmaf(bf_lo(q0), k4[0], s);
+              s = fmaf(bf_hi(q0), k4[1], s);
+              s = fmaf(bf_lo(q1), k4[2], s);
+              s = fmaf(bf_hi(q1), k4[3], s);
+            }
+          s += __shfl_xor(s, 32, LR_WAVE);
+          const float weight = exp2_hw(fmaf(s, c2, nmc));
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4) {
+              const f32x4_t v4 = four(true, page, key, d * 32 + g4 * 8 + half * 4);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[d][4 * g4 + e] = key <= p ? fmaf(weight, v4[e], o[d][4 * g4 + e]) : o[d][4 * g4 + e];
+            }
+        }
+      }
+    }
   }
   if constexpr (KSP == 2) {
     // the second four waves' results to the first four
@@ -1134,7 +1210,6 @@ static int launch_prompt_as(const PagedCache& c, const PagedBatch& t, const Page
 template <int HD, bool E4M3>
 static int launch_prompt(const PagedCache& c, const PagedBatch& t, const PagedQuery& q, void* scratch, hipStream_t s) {
   const PromptPlan p = prompt_plan(c, t, HD, q.rows, q.Hq);
-  if (p.items * p.n_split > (1 << 24)) return LR_E_UNSUPPORTED;   // (workgroups of a grid)
   PagedPrompt a = {q.q, q.ldq, q.y, q.ldy, q.rows, q.Hq, p.n_split, p.bound, q.scale, (float*)scratch, nullptr};
   a.ml_part = a.o_part + (size_t)p.items * p.n_split * PROMPT_ROWS * HD;
   if (p.n_split == 1)
@@ -1147,7 +1222,10 @@ static int launch_prompt(const PagedCache& c, const PagedBatch& t, const PagedQu
 }
 
 static size_t paged_scratch(const PagedCache& c, const PagedBatch& t, int hd, bool e4m3, int rows, int Hq) {
-  if (t.starts) return 256 + prompt_plan(c, t, hd, rows, Hq).bytes;
+  if (t.starts) {
+    const PromptPlan p = prompt_plan(c, t, hd, rows, Hq);
+    return p.items * p.n_split * p.waves > 0xffffffff / 64 ? 0 : 256 + p.bytes;   // (a grid has fewer than 2^32 threads)
+  }
   const DecodePlan p = hd == 128 ? (e4m3 ? decode_plan<128, true>(c, t, Hq) : decode_plan<128, false>(c, t, Hq))
                                  : (e4m3 ? decode_plan<64, true>(c, t, Hq) : decode_plan<64, false>(c, t, Hq));
   if (p.groups > 65535) return 0;   // (a grid's second dimension)
@@ -1173,8 +1251,11 @@ extern "C" int lr_paged_attention(const lr_paged_cache_t* cache, const lr_paged_
   const bool e4m3 = cache->format == LR_CACHE_E4M3;
   if (rows <= 0 || Hq <= 0 || Hq % c.Hkv || (t.starts == nullptr && rows != t.B)) return LR_E_SHAPE;
   if ((int64_t)rows * Hq > 0x3fffffff) return LR_E_UNSUPPORTED;
-  if (Hq > 65535 || ldq < (int64_t)Hq * hd || ldy < (int64_t)Hq * hd || !(scale > 0.0f && scale < INFINITY)) return LR_E_SHAPE;
+  if (Hq > 65535 || ldq < (int64_t)Hq * hd || ldy < (int64_t)Hq * hd) return LR_E_SHAPE;
+  // (the matrix cores give 0 for sums of some 2^-120: a scale that would lift those to numbers that matter is not served)
+  if (!(scale > 0.0f && scale <= 0x1p64f)) return LR_E_SHAPE;
   if (ldq % 8 || ldy % 8) return LR_E_ALIGN;
+  if (paged_overlap(q, ldq, y, ldy, rows, (int64_t)Hq * hd, (int64_t)Hq * hd)) return LR_E_SHAPE;
   const size_t need = paged_scratch(c, t, hd, e4m3, rows, Hq);
   if (need == 0) return LR_E_UNSUPPORTED;
   if (scratch_bytes < need) return LR_E_SHAPE;

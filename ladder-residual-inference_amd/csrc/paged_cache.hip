@@ -240,6 +240,8 @@ extern "C" int lr_paged_write(const lr_paged_cache_t* cache, const lr_paged_batc
   if (rows <= 0 || Hq <= 0 || Hq % c.Hkv || (t.starts == nullptr && rows != t.B)) return LR_E_SHAPE;
   if (Hq > 65535 / 3 || ldqkv < (int64_t)(Hq + 2 * c.Hkv) * hd || ldq < (int64_t)Hq * hd) return LR_E_SHAPE;
   if (ldqkv % 8 || ldq % 8) return LR_E_ALIGN;
+  const bool in_place = q == qkv && (ldq == ldqkv || rows == 1);
+  if (!in_place && paged_overlap(qkv, ldqkv, q, ldq, rows, (int64_t)(Hq + 2 * c.Hkv) * hd, (int64_t)Hq * hd)) return LR_E_SHAPE;
   if (rope && (rope_len <= 0 || rot <= 0 || rot > hd)) return LR_E_SHAPE;
   if (rope && (rot % 16 || (rope_dtype != LR_BF16 && rope_dtype != LR_F32))) return LR_E_UNSUPPORTED;
   const int tokens = paged_tokens(rows, 32);
@@ -267,6 +269,7 @@ extern "C" int lr_paged_read(const lr_paged_cache_t* cache, const lr_paged_batch
   if (rows <= 0 || (t.starts == nullptr && rows != t.B) || c.Hkv > 65535) return LR_E_SHAPE;
   if (ldk < (int64_t)c.Hkv * hd || ldv < (int64_t)c.Hkv * hd) return LR_E_SHAPE;
   if (ldk % 8 || ldv % 8) return LR_E_ALIGN;
+  if (paged_overlap(k, ldk, v, ldv, rows, (int64_t)c.Hkv * hd, (int64_t)c.Hkv * hd)) return LR_E_SHAPE;
   const int tokens = paged_tokens(rows, 4);
   const PagedRead r = {(u16*)k, (u16*)v, ldk, ldv, rows, tokens};
   const dim3 grid((unsigned)((rows + tokens - 1) / tokens));

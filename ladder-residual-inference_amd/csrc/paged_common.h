@@ -55,6 +55,17 @@ __device__ __forceinline__ u32 paged_exponent(float amax) {
 __device__ __forceinline__ float paged_scale(u32 byte) { return __uint_as_float(byte << 23); }
 __device__ __forceinline__ float paged_inverse(u32 byte) { return __uint_as_float((254u - byte) << 23); }
 
+// Whether two matrices of `rows` rows of bf16, a of `wa` and b of `wb` elements each, have memory in common.  Columns of one matrix have not.
+static inline bool paged_overlap(const void* a, int64_t lda, const void* b, int64_t ldb, int rows, int64_t wa, int64_t wb) {
+  typedef __int128 wide;
+  if (rows == 1) lda = ldb = wa > wb ? wa : wb;
+  const wide a0 = (uintptr_t)a, b0 = (uintptr_t)b, a1 = a0 + ((wide)(rows - 1) * lda + wa) * 2, b1 = b0 + ((wide)(rows - 1) * ldb + wb) * 2;
+  if (a1 <= b0 || b1 <= a0) return false;
+  if (lda != ldb) return true;
+  const wide ld = (wide)lda * 2, off = ((b0 - a0) % ld + ld) % ld;   // where b's rows begin in a's
+  return off < wa * 2 || off + wb * 2 > ld;
+}
+
 // Checks of the descriptors that the entry points share; fills the kernels' forms of them.
 static inline int paged_arguments(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, PagedCache& c, PagedBatch& t) {
   if (cache == nullptr || batch == nullptr) return LR_E_NULL;

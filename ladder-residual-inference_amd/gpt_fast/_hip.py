@@ -1406,13 +1406,15 @@ def paged_cache_desc(k, v, scales=None) -> _PagedCache:
 
 def paged_batch_desc(table, lengths, starts=None) -> _PagedBatch:
     """table [B, pages], lengths [B], starts [B + 1] or None: int32 on the device."""
+    load()
     B, pages = table.shape
     assert table.stride(1) == 1 or pages == 1
+    assert table.stride(0) >= pages or B == 1, "a row of the table per sequence: an expanded one has none of its own"
     assert tuple(lengths.shape) == (B,) and lengths.is_contiguous() and lengths.device == table.device
     if starts is not None:
         assert tuple(starts.shape) == (B + 1,) and starts.is_contiguous() and starts.device == table.device
     i = torch.int32
-    d = _PagedBatch(_dev(table, i), max(table.stride(0), pages), _dev(lengths, i), None if starts is None else _dev(starts, i),
+    d = _PagedBatch(_dev(table, i), table.stride(0) if B > 1 else pages, _dev(lengths, i), None if starts is None else _dev(starts, i),
                     device_error_word(table.device).data_ptr(), B, pages)
     d.at = ctypes.addressof(d)
     return d

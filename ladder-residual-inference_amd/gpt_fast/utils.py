@@ -60,19 +60,27 @@ class KVCache(nn.Module):
 
 class PagedBatch:
     """Sequences of one call on paged caches of one shape (PagedKVCache.batch): table, lengths and starts on the device, and the
-    scratch of the attention.  The tensors may be written between calls, also between replays of a captured graph; calls that may overlap
-    have batches of their own."""
+    scratch of the attention.  The tensors may be written between calls, also between replays of a captured graph, and are not replaced;
+    calls that may overlap have batches of their own.  Like any tensor it is made on the current stream, ahead of a capture: work on
+    another stream waits for that one first."""
 
     def __init__(self, cache: "PagedKVCache", table: Tensor, lengths: Tensor, n_head: int, starts: Optional[Tensor], rows: int):
         self.table, self.lengths, self.starts, self.n_head, self.rows = table, lengths, starts, n_head, rows
         self.shape = cache.shape
         assert table.device == cache.k_pages.device, "the tables are where the pages are"
+        if table.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a batch is made ahead of a graph's capture: its scratch is cleared once, and kept")
         self.desc = _hip.paged_batch_desc(table, lengths, starts)
         need = _hip.paged_attention_scratch_bytes(cache.desc(), self.desc, rows, n_head)
         if need == 0:
             raise _hip.LadderHipError(f"a paged cache of pages {cache.shape} is not served with {n_head} q heads and a table "
                                       f"{tuple(table.shape)}: head_dim 64 or 128, pages of 16 to 256 tokens (a power of two)")
         self.scratch = torch.zeros(need, dtype=torch.uint8, device=table.device)
+
+    def __setattr__(self, name, value):
+        if "scratch" in self.__dict__:
+            raise AttributeError(f"a batch's {name} is not replaced: its addresses are kept (write into the tensors, or make another batch)")
+        super().__setattr__(name, value)
 
 
 class PagedKVCache(nn.Module):

@@ -350,6 +350,89 @@ def test_not_a_number_where_it_is_seen(hip):
         assert y[:first].isnan().all() and y[first:].isfinite().all()
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("hq,hkv,hd,page,lengths,new", [
+    (8, 1, 128, 16, [90, 5], [90, 5]), (2, 2, 64, 32, [200], [200]), (4, 1, 128, 64, [700], [700]), (3, 1, 64, 16, [900, 60], [900, 60]),
+    (8, 1, 128, 32, [3000], [65]), (1, 1, 64, 64, [2000], [100]),
+])
+def test_what_later_tokens_hold_does_not_reach_earlier_rows(hip, e4m3, hq, hkv, hd, page, lengths, new):
+    """NaN and infinities in keys and values of a prompt's later tokens, the first of them in the middle of its rows."""
+    weight = PROMPT
+    clean = Case(lengths, hkv, hd, page, e4m3, seed=21, new=new)
+    q = rnd(clean.rows, hq * hd, seed=22)
+    y, spread, size = clean.oracle(q, hq)
+    near = bound(y, spread, size, max(lengths), hd, weight)
+    for back in (1, 2, new[0] // 2, new[0] - 1):
+        case = Case(lengths, hkv, hd, page, e4m3, seed=21, new=new)
+        at = lengths[0] - back                # the first such token
+        for pos in range(at, lengths[0], 3 if back > 2 else 1):
+            p, slot = int(case.table[0, pos // page]), pos % page
+            case.v[p, :, slot, 3] = math.nan
+            if not e4m3:
+                case.v[p, :, slot, hd - 1] = -math.inf
+            if pos % 2:
+                case.k[p, :, slot, 1] = math.nan
+        cache, batch = case.on(DEV, hq)
+        got = cache.attend(batch, q.to(DEV), torch.empty(case.rows, hq * hd, dtype=BF, device=DEV)).cpu().double().view(y.shape)
+        first = new[0] - back                 # the first row that sees it
+        rows = torch.ones(case.rows, dtype=torch.bool)
+        rows[first:new[0]] = False
+        off = ((got - y).abs() / near)[rows]
+        assert not off.isnan().any() and off.max() <= 1, (back, f"{off.max():.2f} of what rounding explains")
+        assert got[first:new[0], :, 3].isnan().all()
+        assert e4m3 or not got[first:new[0], :, hd - 1].isfinite().any()
+
+
+@pytest.mark.parametrize("new", [None, [40, 17]])
+@pytest.mark.parametrize("scale", [1e-37, 1.2e-38, 1e38])
+def test_smallest_and_largest_scales(hip, new, scale):
+    """A scale that makes all weights alike gives means of the values; one beyond 2^64 is refused."""
+    case = Case([100, 77], 1, 64, 16, False, seed=30, new=new)
+    if scale > 1:
+        with pytest.raises(hip.LadderHipError):
+            attend(case, 2, scale=scale)
+    else:
+        attend(case, 2, scale=scale, weight=PROMPT if new else WEIGHT)
+
+
+def test_fewer_rows_than_starts_says(hip):
+    """They are what they are in the whole call, and the others stay as they were."""
+    for e4m3 in (False, True):
+        case = Case([30, 90, 20], 2, 64, 16, e4m3, seed=31, new=[30, 40, 20])
+        cache, batch = case.on(DEV, 4)
+        q = rnd(90, 256, seed=1).to(DEV)
+        whole = cache.attend(batch, q, torch.empty_like(q)).clone()
+        for rows in (1, 29, 30, 31, 69, 71):
+            y = torch.full_like(q, 3)
+            cache.attend(batch, q[:rows], y[:rows])
+            y0, spread, size = case.oracle(q.cpu(), 4)
+            near = bound(y0, spread, size, 90, 64, PROMPT)
+            assert ((y.cpu().double().view(90, 4, 64) - y0).abs() <= near)[:rows].all() and (y[rows:] == 3).all()
+        assert whole.isfinite().all()
+
+
+def test_batches_are_not_changed_under_their_addresses(hip):
+    case = Case([20, 20], 2, 64, 16, False)
+    cache, batch = case.on(DEV, 4)
+    with pytest.raises(AttributeError, match="replaced"):
+        batch.lengths = batch.lengths.clone()
+    with pytest.raises(AssertionError, match="expanded"):
+        cache.batch(batch.table[:1].expand(2, -1), batch.lengths, 4)
+    one = cache.batch(batch.table[:1].expand(1, -1), batch.lengths[:1], 4)      # a single row is its own
+    q = rnd(2, 256).to(DEV)
+    assert torch.equal(cache.attend(one, q[:1], torch.empty_like(q[:1])), cache.attend(batch, q, torch.empty_like(q))[:1])
+    wide = torch.cat([batch.table, batch.table * 0 - 5], 1)                     # rows of a wider table
+    view = cache.batch(wide[:, :batch.table.shape[1]], batch.lengths, 4)
+    assert torch.equal(cache.attend(view, q, torch.empty_like(q)), cache.attend(batch, q, torch.empty_like(q)))
+    graph, x = torch.cuda.CUDAGraph(), torch.zeros(4, device=DEV)
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="capture"):
+            cache.batch(batch.table, batch.lengths, 4)
+    with pytest.raises(hip.LadderHipError):
+        cache.attend(batch, q, q)
+
+
 def test_offsets_beyond_32_bits(hip):
     """Pages whose bytes and whose elements lie beyond 2^32."""
     hq, hkv, hd, page = 8, 8, 128, 256

@@ -80,7 +80,7 @@ def test_arguments_are_checked(hip):
     assert calls(hip, *d, ld=248) == {E_SHAPE} and calls(hip, *d, ld=12 * 128 + 4) == {E_ALIGN}
     assert calls(hip, *d, heads, ld=8) == {E_SHAPE}
     assert calls(hip, *d, heads, Hq=7) == {E_SHAPE}
-    for scale in (0.0, -1.0, math.nan, math.inf):
+    for scale in (0.0, -1.0, math.nan, math.inf, 3e38, 2e19):
         assert calls(hip, *d, (ATTEND,), scale=scale) == {E_SHAPE}
     assert calls(hip, *d, (ATTEND,), scratch_bytes=0) == {E_SHAPE}
     assert calls(hip, *d, (WRITE,), rope=64, rot=144) == {E_SHAPE} and calls(hip, *d, (WRITE,), rope=64, rot=0) == {E_SHAPE}
@@ -138,3 +138,26 @@ def test_the_oracle_places_rows():
     table = torch.tensor([[4, 2, 9], [1, 0, 3]])
     assert O.places(table, [17, 0], None, 16) == [(0, 0, 16, 2, 0)]
     assert O.places(table, [17, 3], [0, 2, 5], 16) == [(0, 0, 15, 4, 15), (1, 0, 16, 2, 0), (2, 1, 0, 1, 0), (3, 1, 1, 1, 1), (4, 1, 2, 1, 2)]
+
+
+def test_operands_that_overlap_are_refused(hip):
+    """(rows, widths of both, their row strides, how far apart in elements) -> whether they share memory; and the calls that check it."""
+    lib, (cache, batch) = hip.load(), descs(hip)
+    c, b = ctypes.byref(cache), ctypes.byref(batch)
+    at, hd, hq = 1 << 20, 128, 8
+    width = (hq + 4) * hd
+    for off, ldq in ((8, width), (hd, hq * hd), (width * 5 - 8, hq * hd), (0, hq * hd), (-8, width), (width, width), (width - 8, 2 * width)):
+        assert lib.lr_paged_write(c, b, at, width, at + 2 * off, ldq, 5, hq, None, 0, 0, 0, 0, None) == E_SHAPE, (off, ldq)
+    for off, ld in ((0, hq * hd), (8, hq * hd), (hq * hd, hq * hd), (-8, 3 * hd * hq), (hq * hd - 8, 3 * hq * hd), (3 * hd * hq - 8, 3 * hd * hq)):
+        assert lib.lr_paged_attention(c, b, at, ld, at + 2 * off, ld, 5, hq, 0.1, 1 << 24, 1 << 30, None) == E_SHAPE, (off, ld)
+    assert lib.lr_paged_attention(c, b, at, hq * hd, at + 2 * hq * hd, 2 * hq * hd, 5, hq, 0.1, 1 << 24, 1 << 30, None) == E_SHAPE
+    for off, ld in ((0, 2 * hd), (8, 2 * hd), (2 * hd - 8, 4 * hd), (-8, 4 * hd)):
+        assert lib.lr_paged_read(c, b, at, ld, at + 2 * off, ld, 5, None) == E_SHAPE, (off, ld)
+
+
+def test_more_workgroups_than_a_launch_has_threads_for(hip):
+    """2^30 rows of q heads: 2^23 workgroups of four waves fit; with as many short sequences as go by a head's blocks on top they do not."""
+    lib = hip.load()
+    size = lambda rows, Hq, **c: (lambda d: lib.lr_paged_attention_scratch_bytes(ctypes.byref(d[0]), ctypes.byref(d[1]), rows, Hq))(descs(hip, **c))
+    assert size(1 << 20, 1 << 10, n_kv_head=1, B=16) > 0
+    assert size(1 << 16, 1 << 10, n_kv_head=1 << 10, B=65535) == 0
