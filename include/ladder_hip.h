@@ -826,13 +826,30 @@ typedef struct lr_paged_batch {
  * (2i, 2i + 1) where interleaved != 0, (i, i + rot / 2) else; products and sums in fp32, each rounded by itself, as lr_rope_kv_write.
  * rot % 16 == 0; rope NULL: nothing is turned.  An e4m3 row is rounded from the fp32 values.  A row whose position or page is out of range is
  * left alone whole, q too.  No two rows may have the same place. */
-int lr_paged_write(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, const void* qkv, int64_t ldqkv, void* q, int64_t ldq,
-                   int rows, int Hq, const void* rope, int rope_len, int rot, int interleaved, int rope_dtype, lr_stream_t stream);
+typedef struct lr_paged_write {
+  const lr_paged_cache_t* cache;
+  const lr_paged_batch_t* batch;
+  const void* qkv;
+  int64_t ldqkv;
+  void* q;
+  int64_t ldq;
+  const void* rope;
+  int32_t rows, Hq, rope_len, rot, interleaved, rope_dtype;
+} lr_paged_write_t;
+int lr_paged_write(const lr_paged_write_t* desc, lr_stream_t stream);
 
 /* The call's tokens back from the cache: k, v [rows, n_kv_head head_dim] bf16 (row strides ldk, ldv), apart from each other.  With starts the running sum of
  * lengths these are whole sequences.  A row whose position or page is out of range is left as it was. */
-int lr_paged_read(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, void* k, int64_t ldk, void* v, int64_t ldv, int rows,
-                  lr_stream_t stream);
+typedef struct lr_paged_read {
+  const lr_paged_cache_t* cache;
+  const lr_paged_batch_t* batch;
+  void* k;
+  int64_t ldk;
+  void* v;
+  int64_t ldv;
+  int32_t rows;
+} lr_paged_read_t;
+int lr_paged_read(const lr_paged_read_t* desc, lr_stream_t stream);
 
 /* y[r, h] = softmax_j( q[r, h] . K[j, h / G] * scale ) V[j, h / G] over the keys j of row r's sequence up to its own position, G =
  * Hq / n_kv_head; q, y [rows, Hq head_dim] (row strides ldq, ldy) with no memory in common.  The cache holds the call's tokens already.
@@ -843,8 +860,19 @@ int lr_paged_read(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, 
  * cache but for its addresses and n_pages, the same B, pages, Hq and starts or none (rows no more than those it was sized for), one
  * after the other: calls that may overlap have their own. */
 size_t lr_paged_attention_scratch_bytes(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, int rows, int Hq);
-int lr_paged_attention(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, const void* q, int64_t ldq, void* y, int64_t ldy,
-                       int rows, int Hq, float scale, void* scratch, size_t scratch_bytes, lr_stream_t stream);
+typedef struct lr_paged_attention {
+  const lr_paged_cache_t* cache;
+  const lr_paged_batch_t* batch;
+  const void* q;
+  int64_t ldq;
+  void* y;
+  int64_t ldy;
+  void* scratch;
+  size_t scratch_bytes;
+  int32_t rows, Hq;
+  float scale;
+} lr_paged_attention_t;
+int lr_paged_attention(const lr_paged_attention_t* desc, lr_stream_t stream);
 
 #ifdef __cplusplus
 }

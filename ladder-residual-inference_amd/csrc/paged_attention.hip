@@ -1239,8 +1239,9 @@ extern "C" size_t lr_paged_attention_scratch_bytes(const lr_paged_cache_t* cache
   return paged_scratch(c, t, cache->head_dim, cache->format == LR_CACHE_E4M3, rows, Hq);
 }
 
-extern "C" int lr_paged_attention(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, const void* q, int64_t ldq, void* y, int64_t ldy,
-                                  int rows, int Hq, float scale, void* scratch, size_t scratch_bytes, lr_stream_t stream) {
+extern "C" int lr_paged_attention(const lr_paged_attention_t* desc, lr_stream_t stream) {
+  if (desc == nullptr) return LR_E_NULL;
+  const auto& [cache, batch, q, ldq, y, ldy, scratch, scratch_bytes, rows, Hq, scale] = *desc;
   PagedCache c;
   PagedBatch t;
   if (const int rc = paged_arguments(cache, batch, c, t)) return rc;

@@ -228,8 +228,9 @@ static void launch_write(bool f32, unsigned grid, const PagedCache& c, const Pag
   else k_paged_write<HD, E4M3, PAIRS, u16><<<dim3(grid), dim3(256), 0, s>>>(c, t, w);
 }
 
-extern "C" int lr_paged_write(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, const void* qkv, int64_t ldqkv, void* q, int64_t ldq,
-                              int rows, int Hq, const void* rope, int rope_len, int rot, int interleaved, int rope_dtype, lr_stream_t stream) {
+extern "C" int lr_paged_write(const lr_paged_write_t* desc, lr_stream_t stream) {
+  if (desc == nullptr) return LR_E_NULL;
+  const auto& [cache, batch, qkv, ldqkv, q, ldq, rope, rows, Hq, rope_len, rot, interleaved, rope_dtype] = *desc;
   PagedCache c;
   PagedBatch t;
   if (const int rc = paged_arguments(cache, batch, c, t)) return rc;
@@ -258,8 +259,9 @@ extern "C" int lr_paged_write(const lr_paged_cache_t* cache, const lr_paged_batc
   return lr_launch_status();
 }
 
-extern "C" int lr_paged_read(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, void* k, int64_t ldk, void* v, int64_t ldv, int rows,
-                             lr_stream_t stream) {
+extern "C" int lr_paged_read(const lr_paged_read_t* desc, lr_stream_t stream) {
+  if (desc == nullptr) return LR_E_NULL;
+  const auto& [cache, batch, k, ldk, v, ldv, rows] = *desc;
   PagedCache c;
   PagedBatch t;
   if (const int rc = paged_arguments(cache, batch, c, t)) return rc;

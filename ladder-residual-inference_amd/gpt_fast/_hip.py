@@ -5,6 +5,7 @@ caller gets an exception.  Tensors are passed as raw device pointers plus sizes;
 torch's current HIP stream, so calls made under torch.cuda.graph() are captured."""
 import ctypes
 import os
+import struct
 from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 import torch
@@ -144,12 +145,10 @@ _PROTOS = {
     "lr_moe_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "lr_moe": (c_int, [c_void_p, c_void_p]),
     "lr_linear_multi_route": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p]),
-    "lr_paged_write": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int,
-                               c_void_p]),
-    "lr_paged_read": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p]),
+    "lr_paged_write": (c_int, [c_void_p, c_void_p]),
+    "lr_paged_read": (c_int, [c_void_p, c_void_p]),
     "lr_paged_attention_scratch_bytes": (c_size_t, [c_void_p, c_void_p, c_int, c_int]),
-    "lr_paged_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_float, c_void_p, c_size_t,
-                                   c_void_p]),
+    "lr_paged_attention": (c_int, [c_void_p, c_void_p]),
 }
 
 
@@ -1420,14 +1419,21 @@ def paged_batch_desc(table, lengths, starts=None) -> _PagedBatch:
     return d
 
 
+# lr_paged_write_t, lr_paged_read_t, lr_paged_attention_t: bytes made in one go and handed over by their address (14 arguments converted one
+# by one are 1.4 us of such a call's 6, this 0.5)
+_PAGED_WRITE = struct.Struct("PPPqPqPiiiiii")
+_PAGED_READ = struct.Struct("PPPqPqi")
+_PAGED_ATTENTION = struct.Struct("PPPqPqPNiif")
+
+
 def _paged_rows(t, width, device):
     """(address, row stride, rows) of a [rows, width] bf16 matrix with dense rows."""
     rows, cols = t.shape
-    ld, unit = t.stride()
+    ld, unit = (cols, 1) if t.is_contiguous() else t.stride()
     if t.dtype is not torch.bfloat16 or cols != width or unit != 1 or t.get_device() != device:
         raise ValueError(f"expected [rows, {width}] bfloat16 with dense rows on cuda:{device}, got {tuple(t.shape)} {t.dtype} "
                          f"with strides {t.stride()} on {t.device}")
-    return t.data_ptr(), (ld if rows > 1 else cols), rows
+    return t.data_ptr(), ld, rows
 
 
 def _paged_stream(device) -> int:
@@ -1438,34 +1444,42 @@ def _paged_stream(device) -> int:
     return torch._C._cuda_getCurrentRawStream(device)
 
 
-def paged_write(cache, batch, qkv, q, n_head, rope=None, interleaved=True):
-    """lr_paged_write: qkv [rows, (n_head + 2 kv heads) head_dim], q [rows, n_head head_dim]; rope [positions, rot / 2, 2] bf16 or fp32."""
+def _paged_most(rows, other, most):
+    if rows != other:
+        raise ValueError(f"{rows} rows of one, {other} of the other")
+    raise ValueError(f"a batch for up to {most} rows: got {rows} rows")
+
+
+def paged_write(cache, batch, qkv, q, n_head, rope=None, interleaved=True, most=0x7fffffff):
+    """lr_paged_write: qkv [rows, (n_head + 2 kv heads) head_dim], q [rows, n_head head_dim]; rope [positions, rot / 2, 2] bf16 or fp32;
+    up to `most` rows."""
     hd, device = cache.head_dim, cache.device
     x, ldx, rows = _paged_rows(qkv, (n_head + 2 * cache.n_kv_head) * hd, device)
     o, ldo, n = _paged_rows(q, n_head * hd, device)
-    if n != rows:
-        raise ValueError(f"{rows} rows of qkv, {n} of q")
-    r, length, rot, kind = None, 0, 0, 0
+    if n != rows or rows > most:
+        _paged_most(rows, n, most)
+    r = length = rot = kind = 0
     if rope is not None:
         length, rot, two = rope.shape
         kind = 0 if rope.dtype is torch.bfloat16 else 1 if rope.dtype is torch.float32 else -1
         if two != 2 or kind < 0 or not rope.is_contiguous() or rope.get_device() != device:
             raise ValueError(f"rope is dense [positions, rot / 2, 2], bfloat16 or float32, on cuda:{device}")
         r, rot = rope.data_ptr(), 2 * rot
-    rc = _lib.lr_paged_write(cache.at, batch.at, x, ldx, o, ldo, rows, n_head, r, length, rot, interleaved, kind, _paged_stream(device))
+    rc = _lib.lr_paged_write(_PAGED_WRITE.pack(cache.at, batch.at, x, ldx, o, ldo, r, rows, n_head, length, rot, interleaved, kind),
+                             _paged_stream(device))
     if rc:
         _check(rc, "lr_paged_write")
     return q
 
 
-def paged_read(cache, batch, k, v):
-    """lr_paged_read: k, v [rows, kv heads * head_dim]."""
+def paged_read(cache, batch, k, v, most=0x7fffffff):
+    """lr_paged_read: k, v [rows, kv heads * head_dim], up to `most` rows."""
     width, device = cache.n_kv_head * cache.head_dim, cache.device
     a, lda, rows = _paged_rows(k, width, device)
     b, ldb, n = _paged_rows(v, width, device)
-    if n != rows:
-        raise ValueError(f"{rows} rows of k, {n} of v")
-    rc = _lib.lr_paged_read(cache.at, batch.at, a, lda, b, ldb, rows, _paged_stream(device))
+    if n != rows or rows > most:
+        _paged_most(rows, n, most)
+    rc = _lib.lr_paged_read(_PAGED_READ.pack(cache.at, batch.at, a, lda, b, ldb, rows), _paged_stream(device))
     if rc:
         _check(rc, "lr_paged_read")
     return k, v
@@ -1475,15 +1489,15 @@ def paged_attention_scratch_bytes(cache, batch, rows, n_head) -> int:
     return int(load().lr_paged_attention_scratch_bytes(cache.at, batch.at, rows, n_head))
 
 
-def paged_attention(cache, batch, q, y, n_head, scratch, scale=None):
-    """lr_paged_attention: q, y [rows, n_head * head_dim]; scratch uint8, zero before the first call."""
+def paged_attention(cache, batch, q, y, n_head, scratch, scale=None, most=0x7fffffff):
+    """lr_paged_attention: q, y [rows, n_head * head_dim], up to `most` rows; scratch (address, bytes), zero before the first call."""
     hd, device = cache.head_dim, cache.device
     x, ldx, rows = _paged_rows(q, n_head * hd, device)
     o, ldo, n = _paged_rows(y, n_head * hd, device)
-    if n != rows:
-        raise ValueError(f"{rows} rows of q, {n} of y")
-    rc = _lib.lr_paged_attention(cache.at, batch.at, x, ldx, o, ldo, rows, n_head, hd ** -0.5 if scale is None else scale, scratch.data_ptr(),
-                                 scratch.numel(), _paged_stream(device))
+    if n != rows or rows > most:
+        _paged_most(rows, n, most)
+    rc = _lib.lr_paged_attention(_PAGED_ATTENTION.pack(cache.at, batch.at, x, ldx, o, ldo, *scratch, rows, n_head,
+                                                       hd ** -0.5 if scale is None else scale), _paged_stream(device))
     if rc:
         _check(rc, "lr_paged_attention")
     return y

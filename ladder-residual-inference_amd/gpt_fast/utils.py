@@ -75,7 +75,9 @@ class PagedBatch:
         if need == 0:
             raise _hip.LadderHipError(f"a paged cache of pages {cache.shape} is not served with {n_head} q heads and a table "
                                       f"{tuple(table.shape)}: head_dim 64 or 128, pages of 16 to 256 tokens (a power of two)")
-        self.scratch = torch.zeros(need, dtype=torch.uint8, device=table.device)
+        scratch = torch.zeros(need, dtype=torch.uint8, device=table.device)
+        self.room = scratch.data_ptr(), need
+        self.scratch = scratch
 
     def __setattr__(self, name, value):
         if "scratch" in self.__dict__:
@@ -144,25 +146,25 @@ class PagedKVCache(nn.Module):
         assert starts is not None or rows in (None, table.shape[0]), "without starts there is one row per sequence"
         return PagedBatch(self, table, lengths, n_head, starts, table.shape[0] if rows is None else rows)
 
-    def _check(self, batch: PagedBatch, rows: int):
+    def _check(self, batch: PagedBatch):
         desc = self._desc or self.desc()
-        if batch.shape != self._shape or rows > batch.rows:
-            raise ValueError(f"a batch for up to {batch.rows} rows and pages {batch.shape}: got {rows} rows, pages {self._shape}")
+        if batch.shape != self._shape:
+            raise ValueError(f"a batch for pages {batch.shape}: got pages {self._shape}")
         return desc
 
     def write(self, batch: PagedBatch, qkv: Tensor, q: Tensor, rope: Optional[Tensor] = None, interleaved: bool = True) -> Tensor:
         """qkv [rows, (n_head + 2 kv heads) head_dim] fresh from the fused projection: q and k rotated by rope [positions, rot / 2, 2]
         (precompute_freqs_cis's table, or fp32; pairs of neighbours, or of the two halves of the first rot dimensions), q to `q` (which may
         be qkv's own columns), k and v into the pages."""
-        return _hip.paged_write(self._check(batch, qkv.shape[0]), batch.desc, qkv, q, batch.n_head, rope, interleaved)
+        return _hip.paged_write(self._check(batch), batch.desc, qkv, q, batch.n_head, rope, interleaved, batch.rows)
 
     def read(self, batch: PagedBatch, k: Tensor, v: Tensor):
         """The call's tokens back, [rows, kv heads * head_dim] bf16."""
-        return _hip.paged_read(self._check(batch, k.shape[0]), batch.desc, k, v)
+        return _hip.paged_read(self._check(batch), batch.desc, k, v, batch.rows)
 
     def attend(self, batch: PagedBatch, q: Tensor, y: Tensor, scale: Optional[float] = None) -> Tensor:
         """y [rows, n_head * head_dim] = attention of the rotated q's rows, each on its sequence's keys up to its own position."""
-        return _hip.paged_attention(self._check(batch, q.shape[0]), batch.desc, q, y, batch.n_head, batch.scratch, scale)
+        return _hip.paged_attention(self._check(batch), batch.desc, q, y, batch.n_head, batch.room, scale, batch.rows)
 
 
 class RMSNorm(nn.Module):

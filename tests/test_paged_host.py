@@ -31,19 +31,36 @@ def descs(hip, **change):
 WRITE, READ, ATTEND = range(3)
 
 
+def address(d):
+    return 0 if d is None else ctypes.addressof(d)
+
+
+def write(hip, cache, batch, qkv, ldqkv, q, ldq, rows, Hq, rope, rope_len, rot, interleaved, rope_dtype):
+    return hip.load().lr_paged_write(hip._PAGED_WRITE.pack(address(cache), address(batch), qkv or 0, ldqkv, q, ldq, rope or 0, rows, Hq, rope_len, rot,
+                                                           interleaved, rope_dtype), None)
+
+
+def read(hip, cache, batch, k, ldk, v, ldv, rows):
+    return hip.load().lr_paged_read(hip._PAGED_READ.pack(address(cache), address(batch), k or 0, ldk, v, ldv, rows), None)
+
+
+def attend(hip, cache, batch, q, ldq, y, ldy, rows, Hq, scale, scratch, scratch_bytes):
+    return hip.load().lr_paged_attention(hip._PAGED_ATTENTION.pack(address(cache), address(batch), q or 0, ldq, y, ldy, scratch, scratch_bytes, rows, Hq,
+                                                                   scale), None)
+
+
 def calls(hip, cache, batch, which=(WRITE, READ, ATTEND), rows=5, Hq=8, ld=None, scale=0.1, x=1 << 20, rope=None, rot=128, rope_dtype=0,
           scratch_bytes=1 << 30):
     """What the entry points `which` return, one value where they agree."""
-    lib, c, b = hip.load(), ctypes.byref(cache), ctypes.byref(batch)
     hd, hkv = max(cache.head_dim, 1), max(cache.n_kv_head, 1)
     width = ld or (Hq + 2 * hkv) * hd
     got = set()
     if WRITE in which:
-        got.add(lib.lr_paged_write(c, b, x, width, 1 << 21, Hq * hd, rows, Hq, rope, 64, rot, 1, rope_dtype, None))
+        got.add(write(hip, cache, batch, x, width, 1 << 21, Hq * hd, rows, Hq, rope, 64, rot, 1, rope_dtype))
     if READ in which:
-        got.add(lib.lr_paged_read(c, b, x, ld or hkv * hd, 1 << 21, ld or hkv * hd, rows, None))
+        got.add(read(hip, cache, batch, x, ld or hkv * hd, 1 << 21, ld or hkv * hd, rows))
     if ATTEND in which:
-        got.add(lib.lr_paged_attention(c, b, x, ld or Hq * hd, 1 << 21, ld or Hq * hd, rows, Hq, scale, 1 << 22, scratch_bytes, None))
+        got.add(attend(hip, cache, batch, x, ld or Hq * hd, 1 << 21, ld or Hq * hd, rows, Hq, scale, 1 << 22, scratch_bytes))
     return got
 
 
@@ -69,10 +86,10 @@ def test_descriptors_are_checked_by_every_entry_point(hip, change, code):
 def test_arguments_are_checked(hip):
     d = descs(hip)
     lib = hip.load()
-    for n in (None,):
-        assert lib.lr_paged_write(n, ctypes.byref(d[1]), 16, 8, 16, 8, 1, 8, None, 0, 0, 0, 0, None) == E_NULL
-        assert lib.lr_paged_read(ctypes.byref(d[0]), n, 16, 8, 16, 8, 1, None) == E_NULL
-        assert lib.lr_paged_attention(n, n, 16, 8, 16, 8, 1, 8, 1.0, 16, 1 << 30, None) == E_NULL
+    assert lib.lr_paged_write(None, None) == lib.lr_paged_read(None, None) == lib.lr_paged_attention(None, None) == E_NULL
+    assert write(hip, None, d[1], 16, 8, 16, 8, 1, 8, None, 0, 0, 0, 0) == E_NULL
+    assert read(hip, d[0], None, 16, 8, 16, 8, 1) == E_NULL
+    assert attend(hip, None, None, 16, 8, 16, 8, 1, 8, 1.0, 16, 1 << 30) == E_NULL
     heads = WRITE, ATTEND
     assert calls(hip, *d, rows=0) == {E_SHAPE}
     assert calls(hip, *d, x=None) == {E_NULL}
@@ -142,17 +159,16 @@ def test_the_oracle_places_rows():
 
 def test_operands_that_overlap_are_refused(hip):
     """(rows, widths of both, their row strides, how far apart in elements) -> whether they share memory; and the calls that check it."""
-    lib, (cache, batch) = hip.load(), descs(hip)
-    c, b = ctypes.byref(cache), ctypes.byref(batch)
+    cache, batch = descs(hip)
     at, hd, hq = 1 << 20, 128, 8
     width = (hq + 4) * hd
     for off, ldq in ((8, width), (hd, hq * hd), (width * 5 - 8, hq * hd), (0, hq * hd), (-8, width), (width, width), (width - 8, 2 * width)):
-        assert lib.lr_paged_write(c, b, at, width, at + 2 * off, ldq, 5, hq, None, 0, 0, 0, 0, None) == E_SHAPE, (off, ldq)
+        assert write(hip, cache, batch, at, width, at + 2 * off, ldq, 5, hq, None, 0, 0, 0, 0) == E_SHAPE, (off, ldq)
     for off, ld in ((0, hq * hd), (8, hq * hd), (hq * hd, hq * hd), (-8, 3 * hd * hq), (hq * hd - 8, 3 * hq * hd), (3 * hd * hq - 8, 3 * hd * hq)):
-        assert lib.lr_paged_attention(c, b, at, ld, at + 2 * off, ld, 5, hq, 0.1, 1 << 24, 1 << 30, None) == E_SHAPE, (off, ld)
-    assert lib.lr_paged_attention(c, b, at, hq * hd, at + 2 * hq * hd, 2 * hq * hd, 5, hq, 0.1, 1 << 24, 1 << 30, None) == E_SHAPE
+        assert attend(hip, cache, batch, at, ld, at + 2 * off, ld, 5, hq, 0.1, 1 << 24, 1 << 30) == E_SHAPE, (off, ld)
+    assert attend(hip, cache, batch, at, hq * hd, at + 2 * hq * hd, 2 * hq * hd, 5, hq, 0.1, 1 << 24, 1 << 30) == E_SHAPE
     for off, ld in ((0, 2 * hd), (8, 2 * hd), (2 * hd - 8, 4 * hd), (-8, 4 * hd)):
-        assert lib.lr_paged_read(c, b, at, ld, at + 2 * off, ld, 5, None) == E_SHAPE, (off, ld)
+        assert read(hip, cache, batch, at, ld, at + 2 * off, ld, 5) == E_SHAPE, (off, ld)
 
 
 def test_more_workgroups_than_a_launch_has_threads_for(hip):
