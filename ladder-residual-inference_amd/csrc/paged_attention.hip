@@ -36,7 +36,7 @@ constexpr int PAGED_OUT = (int)0x80000000;   // an offset outside every resource
 constexpr int PAGED_COHERENT = 17;   // sc0 sc1: past this XCD's L2
 
 __device__ __forceinline__ i32x4_t paged_resource(const u8* at) {
-  return i32x4_t{(int)(u32)(unsigned long long)at, (int)(u32)((unsigned long long)at >> 32) & 0xffff, 0x7fffffff, 0x00020000};
+  return i32x4_t{(int)(u32)(unsigned long long)at, (int)(u32)((unsigned long long)at >> 32), 0x7fffffff, 0x00020000};   // (addresses have 47 bits: no stride)
 }
 // 16 (4) bytes per lane from resource + voff + soff to LDS address `lds` + 16 (4) * lane; counted by vmcnt, not by the compiler
 // (ONCE: rows that nobody else reads, non-temporal)
@@ -765,6 +765,7 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
   // the pages of 16 keys each, 64 of these at a time; which are not there
   const int32_t* const row = t.table + (int64_t)at.b * t.ld_table;
   int pages, groups0;
+  u32 page_lo, page_hi;   // bf16: where the page's rows of this kv head begin
   unsigned long long gone;
   auto ask_pages = [&](int key0) {
     groups0 = key0;
@@ -776,6 +777,11 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
     if (bad && t.err) *t.err = LR_DEV_PAGE_RANGE;
     pages = bad || groups0 + 16 * lane >= t_end ? -1 : pages;
     gone = __ballot(bad);
+    if constexpr (!E4M3) {
+      const int64_t off = paged_offset<RB>(c, pages < 0 ? 0 : pages, kvh);
+      page_lo = (u32)off;
+      page_hi = (u32)(off >> 32);
+    }
   };
   auto pages_from = [&](int key0) {
     ask_pages(key0);
@@ -808,18 +814,23 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
   static_assert(NW * RPL % 16 == 0 && RPL % 4 == 0, "a lane's piece is the same for all of a wave's loads");
   const int kvoff = lrow * RB + (place ^ prompt_k_place<HD>(wave * RPL + lrow)) * 16;
   const int vvoff = lrow * RB + (place ^ prompt_v_place<HD>(lrow)) * 16;
-  auto stage = [&](int t0, int buf) {
+  // (few scalar instructions per load: 150 in all for eight loads were 8 % of the time)
+  auto stage_as = [&](auto WHOLE, int t0, int buf) {
+    const int group0 = (t0 - groups0 + wave * RPL) >> 4;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int first = (i * NW + wave) * RPL;
-      const int page = __builtin_amdgcn_readlane(pages, (t0 - groups0 + first) >> 4);
-      const int64_t off = paged_offset<RB>(c, page < 0 ? 0 : page, kvh);
-      const bool ok = page >= 0 && t0 + first + lrow < t_end;
+      const int first = (i * NW + wave) * RPL, group = group0 + i * NW * RPL / 16;
+      const int64_t off = (int64_t)((unsigned long long)__builtin_amdgcn_readlane(page_hi, group) << 32 | (u32)__builtin_amdgcn_readlane(page_lo, group));
+      const bool ok = WHOLE || (t0 + first + lrow < t_end && !(gone >> group & 1));
       const int soff = ((t0 + first) & ((1 << c.shift) - 1)) * RB;
       const u32 to = lds0 + buf * L::STAGE + (i * NW + wave) * 1024;
       paged_load16(paged_resource(c.k + off), ok ? kvoff : PAGED_OUT, soff, to);
       paged_load16(paged_resource(c.v + off), ok ? vvoff : PAGED_OUT, soff, to + L::TILE);
     }
+  };
+  auto stage = [&](int t0, int buf) {
+    if (t0 + PROMPT_KEYS <= t_end && gone == 0) stage_as(std::true_type{}, t0, buf);
+    else stage_as(std::false_type{}, t0, buf);
   };
   // e4m3: 16 elements of K's or V's rows per piece
   constexpr int NP = 8 * HD / (256 * KSP), HP = HD / 16;

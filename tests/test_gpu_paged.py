@@ -262,6 +262,46 @@ def test_prompts(hip, e4m3, hq, hkv, hd, page, lengths, new):
     attend(Case(lengths, hkv, hd, page, e4m3, seed=7, new=new), hq, weight=PROMPT, behind=3)
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("hd,page,lengths,new", [
+    (128, 16, [(37 * b) % 150 for b in range(90)], [min((37 * b) % 150, 1 + b % 7) for b in range(90)]),
+    (64, 32, [5] * 100, [b % 12 for b in range(100)]),                                                      # many of them see no key at all
+    (64, 64, [1100, 0, 700, 1], [90, 0, 400, 1]),
+    (128, 32, [1300, 20], [1300, 20]),
+])
+def test_prompts_of_many_blocks(hip, e4m3, hd, page, lengths, new):
+    """More than the chip holds at once, most of them short; the same bits again, also replayed."""
+    hq, hkv = (16, 8) if len(lengths) > 10 else (32, 16)
+    case = Case(lengths, hkv, hd, page, e4m3, seed=41, new=new)
+    if len(lengths) > 10:
+        cache, batch, q, got = attend(case, hq, weight=PROMPT, behind=2)
+    else:
+        cache, batch = case.on(DEV, hq)
+        q = rnd(case.rows, hq * hd, seed=1)
+    x = q.to(DEV)
+    y = torch.full_like(x, 3)
+    cache.attend(batch, x, y)
+    want = y.clone()
+    # against one sequence at a time, whose blocks are few
+    for b, n in enumerate(new):
+        if n:
+            i = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)
+            one = cache.batch(batch.table[b:b + 1], batch.lengths[b:b + 1], hq, starts=i(0, n), rows=n)
+            at = slice(case.starts[b], case.starts[b] + n)
+            off = (cache.attend(one, x[at], torch.empty_like(x[at])).float() - want[at].float()).abs()
+            assert off.max() <= 2.0 ** -6 * 4 and want[at].isfinite().all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.attend(batch, x, y)
+    for _ in range(5):
+        y.fill_(3)
+        cache.attend(batch, x, y)
+        assert torch.equal(y, want)
+        y.fill_(3)
+        graph.replay()
+        assert torch.equal(y, want)
+
+
 def test_rows_ahead_of_a_sequences_first_token_see_nothing(hip):
     """More rows than tokens: those at negative positions are zeros."""
     for e4m3 in (False, True):
