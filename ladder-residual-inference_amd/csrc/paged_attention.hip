@@ -27,7 +27,12 @@ struct PagedQuery {
 // (16x16x32, up to 16 q heads of the kv head are the columns): a lane holds eight scores of one head and, since the order of keys in a product
 // is free, hands them on as the second product's operand without moving them.  Weights enter as two bf16 numbers (2^-16 of the
 // weight).  e4m3: K is expanded with its row's power of two on the way to the product, V without, its power goes into the weight.
-// Bound: memory.
+//
+// Bound: memory.  64 sequences of 2048 keys, 8 kv heads of 128, e4m3: 43.4 us, 6.3 TB/s (a plain read 7.0); one of 131072 in bf16 85.5 us, 6.3 TB/s;
+// 24 of 1 to 4096 27.4 us.  One workgroup per CU with four waves whose tiles are all in flight reads faster than two or three smaller ones (the first
+// of these 43.6, 50, 58), rows that nobody else reads come non-temporally (10 %).  Few keys: a chain of waits, 8.4 us for one sequence of 2048
+// and one kv head: the lengths 0.7, page numbers and q 1.1, keys, values and products 1.5, four waves' results 0.9, what a worker leaves
+// and its ticket 1.0, the parts together 1.8, the rest the launch.
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -656,9 +661,16 @@ static int launch_paged_decode(const PagedCache& c, const PagedBatch& t, const P
 //   S^T[key][row] = K q^T,   O^T[dim][row] += V^T P^T
 // on the matrix cores (32x32x16).  A column is a lane, so maxima, sums and factors are a lane's own, and the 16 scores that it holds of 32 keys are, in
 // their order, the second product's operand.  Weights enter as one bf16 number: y is off by their rounding, at most 2^-8 of each and at random,
-// where keys are many about as much as by y's own rounding (1.41 times the error of exact sums rounded).  Keys come 64 at a time into one of two buffers, one barrier per 64; bf16 by loads straight into LDS, e4m3 through registers, expanded on
-// the way with its row's power of two: from there on the two are the same.
+// where keys are many about as much as by y's own rounding (1.41 times the error of exact sums rounded).  Keys come 64 at a time into one of
+// two buffers, one barrier per 64; bf16 by loads straight into LDS, e4m3 through registers, expanded on the way with its row's power of two:
+// from there on the two are the same.
 // Few rows: a workgroup's keys are cut among several, whose results a second launch puts together.
+//
+// Bound: the waves' instructions, one after another: 32 products of 32 cycles, 32 exponentials of 16 and some 250 others of 4 or more per wave
+// and 64 keys; two waves a SIMD (222 registers) hide little more of one another than this.  Five prompts of up to 2048 tokens, 32 q and 8 kv heads of
+// 128: 135 to 141 us, 0.82 PFLOP/s of the 1.35 of a large library product; without what a workgroup does once (its block looked up, q,
+// the first portion, the rows stored; 6.7 us) 109.  Slower: products and exponentials of two tiles interleaved (137 -> 140), two groups of waves in
+// turn (26.8 -> 28.4 for the 256 tokens behind 8000 that take 26.5), workgroups that take several blocks (the registers spill: 138 -> 146).
 constexpr int PROMPT_ROWS = 128, PROMPT_KEYS = 64;
 constexpr int PROMPT_SPLIT_KEYS = 256;   // a part of a row's keys has at least so many
 
@@ -814,7 +826,7 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
   static_assert(NW * RPL % 16 == 0 && RPL % 4 == 0, "a lane's piece is the same for all of a wave's loads");
   const int kvoff = lrow * RB + (place ^ prompt_k_place<HD>(wave * RPL + lrow)) * 16;
   const int vvoff = lrow * RB + (place ^ prompt_v_place<HD>(lrow)) * 16;
-  // (few scalar instructions per load: 150 in all for eight loads were 8 % of the time)
+  // (with few scalar instructions per load, which a wave issues one by one beside everything else: 150 for the eight of a portion, now 70; 143.5 -> 141 us)
   auto stage_as = [&](auto WHOLE, int t0, int buf) {
     const int group0 = (t0 - groups0 + wave * RPL) >> 4;
 #pragma unroll
