@@ -2,7 +2,7 @@
 //
 // Both move every byte once and compute next to nothing: memory-bound, and in a decode step bound by the launch and two dependent
 // reads (where the row belongs, then its page).  A lane has 8 elements of a head's row (16 bytes of bf16), HD / 8 lanes a row.
-// Six prompts of the 8B model into e4m3, 111 MB: 24.4 us, 4.5 TB/s (a large copy 5.05); 16 sequences of it read back, 116 MB: 21.2 us, 5.5 TB/s; a row of
+// Six prompts of the 8B model into e4m3, 110 MB: 23.3 us, 4.7 TB/s (a large copy 5.05); 16 sequences of it read back, 116 MB: 21.2 us, 5.5 TB/s; a row of
 // one sequence, or of 64: 5.2 us from Python, most of it the call.
 #include "paged_common.h"
 
@@ -71,20 +71,40 @@ struct PagedWrite {
   int rope_len, rot, rows, Hq, tokens;
 };
 
-// x[lo] c - x[hi] s and x[hi] c + x[lo] s for the 8 elements from d on, each product rounded by itself (as lr_rope_kv_write does it).
-// PAIRS: a pair is two neighbours; else element i and i + rot / 2, whose 8 are read besides.
+// The angles that a lane's 8 elements from d on take, (cos, sin) pairs as they lie: 4 of them where a pair is two neighbours (PAIRS), else 8, of
+// element i and i + rot / 2.
 template <bool PAIRS, typename T>
-__device__ __forceinline__ void paged_turn(float* f, const u16* row, int d, const T* angles, int rot) {
-#pragma clang fp contract(off)
-  const int half = rot >> 1;
-  if constexpr (PAIRS) {
-    float t[8];
-    if constexpr (sizeof(T) == 2) {
-      unpack8(ld16(angles + d), t);
-    } else {
-      *reinterpret_cast<float4*>(t) = *reinterpret_cast<const float4*>(angles + d);
-      *reinterpret_cast<float4*>(t + 4) = *reinterpret_cast<const float4*>(angles + d + 4);
+struct PagedAngles {
+  static constexpr int N = PAIRS ? 8 : 16, LOADS = N * (int)sizeof(T) / 16;
+  uint4 raw[LOADS];
+  __device__ __forceinline__ void load(const void* rope, int pos, int rot, int d) {
+    const T* const from = (const T*)rope + (int64_t)pos * rot + (PAIRS ? d : 2 * (d >= rot >> 1 ? d - (rot >> 1) : d));
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) raw[i] = ld16(reinterpret_cast<const unsigned char*>(from) + 16 * i);
+  }
+  __device__ __forceinline__ void values(float* t) const {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        unpack8(raw[i], t + 8 * i);
+      } else {
+        t[4 * i] = __uint_as_float(raw[i].x);
+        t[4 * i + 1] = __uint_as_float(raw[i].y);
+        t[4 * i + 2] = __uint_as_float(raw[i].z);
+        t[4 * i + 3] = __uint_as_float(raw[i].w);
+      }
     }
+  }
+};
+
+// x[lo] c - x[hi] s and x[hi] c + x[lo] s for the 8 elements x from d on, each product rounded by itself (as lr_rope_kv_write does it).  The other
+// halves are rot / 16 lanes away.
+template <bool PAIRS, typename T>
+__device__ __forceinline__ void paged_turn(float* f, const uint4& x, int d, const PagedAngles<PAIRS, T>& angles, int rot) {
+#pragma clang fp contract(off)
+  float t[PagedAngles<PAIRS, T>::N];
+  angles.values(t);
+  if constexpr (PAIRS) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float a = f[2 * i], b = f[2 * i + 1], c = t[2 * i], s = t[2 * i + 1];
@@ -92,17 +112,10 @@ __device__ __forceinline__ void paged_turn(float* f, const u16* row, int d, cons
       f[2 * i + 1] = b * c + a * s;
     }
   } else {
-    const bool second = d >= half;
-    const int i0 = second ? d - half : d;
-    float o[8], t[16];
-    unpack8(ld16(row + (second ? d - half : d + half)), o);
-    if constexpr (sizeof(T) == 2) {
-      unpack8(ld16(angles + 2 * i0), t);
-      unpack8(ld16(angles + 2 * i0 + 8), t + 8);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(t + 4 * j) = *reinterpret_cast<const float4*>(angles + 2 * i0 + 4 * j);
-    }
+    const bool second = d >= rot >> 1;
+    const int from = (int)(threadIdx.x & 63) + (second ? -(rot >> 4) : rot >> 4);
+    float o[8];
+    unpack8(make_uint4(__shfl(x.x, from, 64), __shfl(x.y, from, 64), __shfl(x.z, from, 64), __shfl(x.w, from, 64)), o);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float p = f[j] * t[2 * j], r = o[j] * t[2 * j + 1];
@@ -118,12 +131,19 @@ __global__ __launch_bounds__(256) void k_paged_write(const PagedCache c, const P
   paged_places(c, t, row0, w.rows, w.tokens, w.rope ? w.rope_len : 0x7fffffff, at);
   constexpr int LANES = HD / 8, ROWS = 256 / LANES;
   const int heads = w.Hq + 2 * c.Hkv, d = threadIdx.x % LANES * 8, n = w.tokens * heads;
+  PagedAngles<PAIRS, T> angles;   // of token `turned`, asked for behind its first rows: once for all heads (six prompts, by halves in fp32: 33.1 -> 25.5 us)
+  int turned = -1;
   for (int i0 = threadIdx.x / LANES; i0 < n; i0 += ROWS * PAGED_AHEAD) {   // (all lanes of a row go round together)
     uint4 x[PAGED_AHEAD];
 #pragma unroll
     for (int u = 0; u < PAGED_AHEAD; ++u) {
       const int i = i0 + u * ROWS < n ? i0 + u * ROWS : i0, token = i / heads, head = i - token * heads;
       x[u] = ld16_once(w.x + (at.page[token] >= 0 ? row0 + token : 0) * w.ldx + head * HD + d);
+    }
+    const int token0 = i0 / heads;
+    if (w.rope && d < w.rot && turned != token0 && at.page[token0] >= 0) {
+      angles.load(w.rope, at.pos[token0], w.rot, d);
+      turned = token0;
     }
 #pragma unroll
     for (int u = 0; u < PAGED_AHEAD; ++u) {
@@ -134,8 +154,13 @@ __global__ __launch_bounds__(256) void k_paged_write(const PagedCache c, const P
       const int pos = at.pos[token];
       float f[8];
       unpack8(x[u], f);
-      if (w.rope && head < w.Hq + c.Hkv && d < w.rot)
-        paged_turn<PAIRS>(f, w.x + (row0 + token) * w.ldx + head * HD, d, (const T*)w.rope + (int64_t)pos * w.rot, w.rot);
+      if (w.rope && head < w.Hq + c.Hkv && d < w.rot) {
+        if (turned != token) {
+          angles.load(w.rope, pos, w.rot, d);
+          turned = token;
+        }
+        paged_turn(f, x[u], d, angles, w.rot);
+      }
       if (head < w.Hq) {
         // (qkv and q non-temporal: 26.7 -> 24.4 us of those prompts.  k and v are not: 23.2, but the attention behind it 16 us longer)
         const uint4 o = pack8(f);
@@ -216,12 +241,13 @@ __global__ __launch_bounds__(256) void k_paged_read(const PagedCache c, const Pa
   }
 }
 
-// Tokens of a workgroup, which share the search for their places: as many as leave each of 256 CUs so many workgroups.  us, 6 prompts of the 8B
-// model into e4m3 with 4 and with 1 token: 28.3, 26.7 (48 rows of q, k and v per token); 16 sequences of it read back with 16, 9 and 4: 27.5,
-// 27.5, 29.2 (16 rows).
-static inline int paged_tokens(int rows, int per_cu) {
+// Tokens of a workgroup, which share the search for their places: as many as leave each of 256 CUs so many workgroups, and give a lane of a write no more
+// than the rows that it asks for at once.  us, 6 prompts of the 8B model (48 rows of q, k and v per token) written with 4 and with 1 token: 26.1, 23.5; 4 of
+// the 70B model's rank shard (10 rows) with 4 and with 1: 11.2, 14.6; 16 sequences of the 8B model read back (16 rows) with 16, 9 and 4: 27.5, 27.5, 29.2.
+static inline int paged_tokens(int rows, int per_cu, int most) {
   const int n = rows / (per_cu * 256);
-  return n < 1 ? 1 : n > PAGED_TOKENS ? PAGED_TOKENS : n;
+  most = most < PAGED_TOKENS ? most : PAGED_TOKENS;
+  return n < 1 || most < 1 ? 1 : n > most ? most : n;
 }
 
 template <int HD, bool E4M3, bool PAIRS>
@@ -247,7 +273,7 @@ extern "C" int lr_paged_write(const lr_paged_write_t* desc, lr_stream_t stream) 
   if (!in_place && paged_overlap(qkv, ldqkv, q, ldq, rows, (int64_t)(Hq + 2 * c.Hkv) * hd, (int64_t)Hq * hd)) return LR_E_SHAPE;
   if (rope && (rope_len <= 0 || rot <= 0 || rot > hd)) return LR_E_SHAPE;
   if (rope && (rot % 16 || (rope_dtype != LR_BF16 && rope_dtype != LR_F32))) return LR_E_UNSUPPORTED;
-  const int tokens = paged_tokens(rows, 32);
+  const int tokens = paged_tokens(rows, 8, 256 / (hd / 8) * PAGED_AHEAD / (Hq + 2 * c.Hkv));
   const PagedWrite w = {(const u16*)qkv, ldqkv, (u16*)q, ldq, rope, rope_len, rot, rows, Hq, tokens};
   const unsigned grid = (unsigned)((rows + tokens - 1) / tokens);
   const bool f32 = rope_dtype == LR_F32;
@@ -274,7 +300,7 @@ extern "C" int lr_paged_read(const lr_paged_read_t* desc, lr_stream_t stream) {
   if (ldk < (int64_t)c.Hkv * hd || ldv < (int64_t)c.Hkv * hd) return LR_E_SHAPE;
   if (ldk % 8 || ldv % 8) return LR_E_ALIGN;
   if (paged_overlap(k, ldk, v, ldv, rows, (int64_t)c.Hkv * hd, (int64_t)c.Hkv * hd)) return LR_E_SHAPE;
-  const int tokens = paged_tokens(rows, 4);
+  const int tokens = paged_tokens(rows, 4, PAGED_TOKENS);
   const PagedRead r = {(u16*)k, (u16*)v, ldk, ldv, rows, tokens};
   const dim3 grid((unsigned)((rows + tokens - 1) / tokens));
   hipStream_t s = (hipStream_t)stream;
