@@ -7,7 +7,8 @@
 #include "paged_common.h"
 
 constexpr int PAGED_TOKENS = 16;   // of a workgroup, at most
-constexpr int PAGED_AHEAD = 4;     // rows that a lane asks for before it works on the first
+constexpr int PAGED_AHEAD = 4;     // rows that a lane of a write asks for before it works on the first (two: four prompts of the 70B model's shard 8.4 -> 9.3 us)
+constexpr int PAGED_AHEAD_READ = 2;   // of a read (four: 333 tokens of 8 heads of 64 2.7 -> 3.2 us)
 
 // Where a workgroup's tokens belong.  page -1: the token is left alone.
 struct PagedPlace {
@@ -203,11 +204,11 @@ __global__ __launch_bounds__(256) void k_paged_read(const PagedCache c, const Pa
   paged_places(c, t, row0, r.rows, r.tokens, 0x7fffffff, at);
   constexpr int LANES = HD / 8, ROWS = 256 / LANES;
   const int d = threadIdx.x % LANES * 8, n = r.tokens * 2 * c.Hkv;
-  for (int i0 = threadIdx.x / LANES; i0 < n; i0 += ROWS * PAGED_AHEAD) {
-    uint4 x[PAGED_AHEAD];   // (e4m3: eight bytes)
-    u32 byte[PAGED_AHEAD];
+  for (int i0 = threadIdx.x / LANES; i0 < n; i0 += ROWS * PAGED_AHEAD_READ) {
+    uint4 x[PAGED_AHEAD_READ];   // (e4m3: eight bytes)
+    u32 byte[PAGED_AHEAD_READ];
 #pragma unroll
-    for (int u = 0; u < PAGED_AHEAD; ++u) {
+    for (int u = 0; u < PAGED_AHEAD_READ; ++u) {
       const int i = i0 + u * ROWS < n ? i0 + u * ROWS : i0, token = i / (2 * c.Hkv), j = i - token * 2 * c.Hkv, value = j >= c.Hkv, kvh = j - value * c.Hkv;
       const int page = at.page[token] < 0 ? 0 : at.page[token], slot = at.page[token] < 0 ? 0 : at.pos[token] & ((1 << c.shift) - 1);
       const u8* const from = (value ? c.v : c.k) + paged_offset<HD * (E4M3 ? 1 : 2)>(c, page, kvh);
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(256) void k_paged_read(const PagedCache c, const Pa
       }
     }
 #pragma unroll
-    for (int u = 0; u < PAGED_AHEAD; ++u) {
+    for (int u = 0; u < PAGED_AHEAD_READ; ++u) {
       const int i = i0 + u * ROWS;
       if (i >= n) break;
       const int token = i / (2 * c.Hkv), j = i - token * 2 * c.Hkv, value = j >= c.Hkv, kvh = j - value * c.Hkv;
@@ -243,7 +244,7 @@ __global__ __launch_bounds__(256) void k_paged_read(const PagedCache c, const Pa
 
 // Tokens of a workgroup, which share the search for their places: as many as leave each of 256 CUs so many workgroups, and give a lane of a write no more
 // than the rows that it asks for at once.  us, 6 prompts of the 8B model (48 rows of q, k and v per token) written with 4 and with 1 token: 26.1, 23.5; 4 of
-// the 70B model's rank shard (10 rows) with 4 and with 1: 11.2, 14.6; 16 sequences of the 8B model read back (16 rows) with 16, 9 and 4: 27.5, 27.5, 29.2.
+// the 70B model's rank shard (10 rows) with 6, 4 and 1: 8.4, 11.2, 14.6; 16 sequences of the 8B model read back (16 rows) with 16, 9 and 4: 27.5, 27.5, 29.2.
 static inline int paged_tokens(int rows, int per_cu, int most) {
   const int n = rows / (per_cu * 256);
   most = most < PAGED_TOKENS ? most : PAGED_TOKENS;
@@ -273,7 +274,7 @@ extern "C" int lr_paged_write(const lr_paged_write_t* desc, lr_stream_t stream) 
   if (!in_place && paged_overlap(qkv, ldqkv, q, ldq, rows, (int64_t)(Hq + 2 * c.Hkv) * hd, (int64_t)Hq * hd)) return LR_E_SHAPE;
   if (rope && (rope_len <= 0 || rot <= 0 || rot > hd)) return LR_E_SHAPE;
   if (rope && (rot % 16 || (rope_dtype != LR_BF16 && rope_dtype != LR_F32))) return LR_E_UNSUPPORTED;
-  const int tokens = paged_tokens(rows, 8, 256 / (hd / 8) * PAGED_AHEAD / (Hq + 2 * c.Hkv));
+  const int tokens = paged_tokens(rows, 2, 256 / (hd / 8) * PAGED_AHEAD / (Hq + 2 * c.Hkv));
   const PagedWrite w = {(const u16*)qkv, ldqkv, (u16*)q, ldq, rope, rope_len, rot, rows, Hq, tokens};
   const unsigned grid = (unsigned)((rows + tokens - 1) / tokens);
   const bool f32 = rope_dtype == LR_F32;
