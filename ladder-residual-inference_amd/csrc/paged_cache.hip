@@ -2,7 +2,7 @@
 //
 // Both move every byte once and compute next to nothing: memory-bound, and in a decode step bound by the launch and two dependent
 // reads (where the row belongs, then its page).  A lane has 8 elements of a head's row (16 bytes of bf16), HD / 8 lanes a row.
-// Six prompts of the 8B model into e4m3, 110 MB: 23.3 us, 4.7 TB/s (a large copy 5.05); 16 sequences of it read back, 116 MB: 21.2 us, 5.5 TB/s; a row of
+// Six prompts of the 8B model into e4m3, 110 MB: 23.3 us, 4.7 TB/s (a large copy 5.05); 16 sequences of it read back, 116 MB: 20.1 us, 5.8 TB/s; a row of
 // one sequence, or of 64: 5.2 us from Python, most of it the call.
 #include "paged_common.h"
 
@@ -235,19 +235,19 @@ __global__ __launch_bounds__(256) void k_paged_read(const PagedCache c, const Pa
         o.z = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[u].y, s, false));
         o.w = __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[u].y, s, true));
       }
-      // (non-temporal: 16 sequences of the 8B model from e4m3, 116 MB, 27.5 -> 21.2 us)
+      // (non-temporal: those 16 sequences 27.5 -> 21.2 us)
       u16* const to = (value ? r.v + (row0 + token) * r.ldv : r.k + (row0 + token) * r.ldk) + kvh * HD + d;
       __builtin_nontemporal_store(u32x4_t{o.x, o.y, o.z, o.w}, reinterpret_cast<u32x4_t*>(to));
     }
   }
 }
 
-// Tokens of a workgroup, which share the search for their places: as many as leave each of 256 CUs so many workgroups, and give a lane of a write no more
-// than the rows that it asks for at once.  us, 6 prompts of the 8B model (48 rows of q, k and v per token) written with 4 and with 1 token: 26.1, 23.5; 4 of
-// the 70B model's rank shard (10 rows) with 6, 4 and 1: 8.4, 11.2, 14.6; 16 sequences of the 8B model read back (16 rows) with 16, 9 and 4: 27.5, 27.5, 29.2.
-static inline int paged_tokens(int rows, int per_cu, int most) {
-  const int n = rows / (per_cu * 256);
-  most = most < PAGED_TOKENS ? most : PAGED_TOKENS;
+// Tokens of a workgroup, which share the search for their places: as many as its lanes ask for at once (`heads` rows of a token), where that leaves each of
+// 256 CUs two workgroups.  us, 6 prompts of the 8B model (48 rows of q, k and v per token) written with 1, 2 and 4 tokens: 23.5, 26.1, 27.3; 4 of
+// the 70B model's rank shard (10 rows) with 1, 4, 6 and 12: 14.6, 11.2, 8.4, 11.8; 16 sequences of the 8B model read back (16 rows) with 2, 4 and 8: 20.1, 20.1, 22.1.
+template <int AHEAD>
+static inline int paged_tokens(int rows, int heads, int hd) {
+  const int n = rows / (2 * 256), fit = 256 / (hd / 8) * AHEAD / heads, most = fit < PAGED_TOKENS ? fit : PAGED_TOKENS;
   return n < 1 || most < 1 ? 1 : n > most ? most : n;
 }
 
@@ -274,7 +274,7 @@ extern "C" int lr_paged_write(const lr_paged_write_t* desc, lr_stream_t stream) 
   if (!in_place && paged_overlap(qkv, ldqkv, q, ldq, rows, (int64_t)(Hq + 2 * c.Hkv) * hd, (int64_t)Hq * hd)) return LR_E_SHAPE;
   if (rope && (rope_len <= 0 || rot <= 0 || rot > hd)) return LR_E_SHAPE;
   if (rope && (rot % 16 || (rope_dtype != LR_BF16 && rope_dtype != LR_F32))) return LR_E_UNSUPPORTED;
-  const int tokens = paged_tokens(rows, 2, 256 / (hd / 8) * PAGED_AHEAD / (Hq + 2 * c.Hkv));
+  const int tokens = paged_tokens<PAGED_AHEAD>(rows, Hq + 2 * c.Hkv, hd);
   const PagedWrite w = {(const u16*)qkv, ldqkv, (u16*)q, ldq, rope, rope_len, rot, rows, Hq, tokens};
   const unsigned grid = (unsigned)((rows + tokens - 1) / tokens);
   const bool f32 = rope_dtype == LR_F32;
@@ -301,7 +301,7 @@ extern "C" int lr_paged_read(const lr_paged_read_t* desc, lr_stream_t stream) {
   if (ldk < (int64_t)c.Hkv * hd || ldv < (int64_t)c.Hkv * hd) return LR_E_SHAPE;
   if (ldk % 8 || ldv % 8) return LR_E_ALIGN;
   if (paged_overlap(k, ldk, v, ldv, rows, (int64_t)c.Hkv * hd, (int64_t)c.Hkv * hd)) return LR_E_SHAPE;
-  const int tokens = paged_tokens(rows, 4, PAGED_TOKENS);
+  const int tokens = paged_tokens<PAGED_AHEAD_READ>(rows, 2 * c.Hkv, hd);
   const PagedRead r = {(u16*)k, (u16*)v, ldk, ldv, rows, tokens};
   const dim3 grid((unsigned)((rows + tokens - 1) / tokens));
   hipStream_t s = (hipStream_t)stream;
