@@ -777,7 +777,7 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
   // the pages of 16 keys each, 64 of these at a time; which are not there
   const int32_t* const row = t.table + (int64_t)at.b * t.ld_table;
   int pages, groups0;
-  u32 page_lo, page_hi;   // bf16: where the page's rows of this kv head begin
+  u32 page_lo, page_hi;   // bf16: where the page's rows of this kv head begin (e4m3 has the page's number times the kv heads and its own in `pages`)
   unsigned long long gone;
   auto ask_pages = [&](int key0) {
     groups0 = key0;
@@ -789,11 +789,10 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
     if (bad && t.err) *t.err = LR_DEV_PAGE_RANGE;
     pages = bad || groups0 + 16 * lane >= t_end ? -1 : pages;
     gone = __ballot(bad);
-    if constexpr (!E4M3) {
-      const int64_t off = paged_offset<RB>(c, pages < 0 ? 0 : pages, kvh);
-      page_lo = (u32)off;
-      page_hi = (u32)(off >> 32);
-    }
+    const int64_t off = paged_offset<RB>(c, pages < 0 ? 0 : pages, kvh);
+    page_lo = (u32)off;
+    page_hi = (u32)(off >> 32);
+    pages = pages < 0 ? -1 : paged_index(c, pages, kvh);
   };
   auto pages_from = [&](int key0) {
     ask_pages(key0);
@@ -852,11 +851,11 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int x = i * 256 * KSP + tid, value = x >= 4 * HD, key = x % (4 * HD) / HP, pc = x % HP;
-      const int page = __shfl(pages, (t0 - groups0 + key) >> 4, 64);
-      const bool ok = page >= 0 && t0 + key < t_end;
-      const int slot = (t0 + key) & ((1 << c.shift) - 1), safe = ok ? page : 0;
-      raw[i] = ld16((value ? c.v : c.k) + paged_offset<HD>(c, safe, kvh) + slot * HD + pc * 16);
-      byte[i] = c.scales[paged_scales(c, safe, kvh) + (value << c.shift) + slot];
+      const int index = __shfl(pages, (t0 - groups0 + key) >> 4, 64);
+      const bool ok = index >= 0 && t0 + key < t_end;
+      const int slot = (t0 + key) & ((1 << c.shift) - 1), safe = ok ? index : 0;
+      raw[i] = ld16((value ? c.v : c.k) + paged_offset<HD>(c, safe) + slot * HD + pc * 16);
+      byte[i] = c.scales[paged_scales(c, safe) + (value << c.shift) + slot];
       if (!ok) raw[i] = make_uint4(0, 0, 0, 0), byte[i] = 127;
     }
   };

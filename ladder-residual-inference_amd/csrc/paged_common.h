@@ -36,13 +36,15 @@ __device__ __forceinline__ int paged_sums(int v) {
   return v;
 }
 
-// Bytes from the start of k, v to (page, kv head, slot 0)
+// (page, kv head) as one number of 32 bits, and the bytes from the start of k, v to its slot 0
+__device__ __forceinline__ int paged_index(const PagedCache& c, int page, int head) { return page * c.Hkv + head; }
 template <int ROW>
-__device__ __forceinline__ int64_t paged_offset(const PagedCache& c, int page, int head) {
-  return (((int64_t)page * c.Hkv + head) << c.shift) * ROW;
-}
+__device__ __forceinline__ int64_t paged_offset(const PagedCache& c, int index) { return ((int64_t)index << c.shift) * ROW; }
+template <int ROW>
+__device__ __forceinline__ int64_t paged_offset(const PagedCache& c, int page, int head) { return paged_offset<ROW>(c, paged_index(c, page, head)); }
 // and of the scales, to those of the page's keys; its values' follow
-__device__ __forceinline__ int64_t paged_scales(const PagedCache& c, int page, int head) { return ((int64_t)page * c.Hkv + head) << (c.shift + 1); }
+__device__ __forceinline__ int64_t paged_scales(const PagedCache& c, int index) { return (int64_t)index << (c.shift + 1); }
+__device__ __forceinline__ int64_t paged_scales(const PagedCache& c, int page, int head) { return paged_scales(c, paged_index(c, page, head)); }
 
 // An 8-bit row holds x / 2^e as e4m3, e the smallest exponent with max|x| <= 448 * 2^e, kept as the byte e + 127.  A power of two: dividing
 // and multiplying by it rounds nothing, so a value is rounded once, and what is read back is exact in bf16.  (amax: the largest finite
@@ -79,7 +81,8 @@ static inline int paged_arguments(const lr_paged_cache_t* cache, const lr_paged_
   if (cache->format == LR_CACHE_E4M3) LR_REQUIRE_PTR(cache->scales);
   if (cache->head_dim != 64 && cache->head_dim != 128) return LR_E_UNSUPPORTED;
   if (cache->page < 16 || cache->page > 256 || (cache->page & (cache->page - 1))) return LR_E_UNSUPPORTED;
-  // (positions, and tiles of 32 keys of all sequences, are 32-bit numbers)
+  // (positions, tiles of 32 keys of all sequences, and pages times heads are 32-bit numbers)
+  if ((int64_t)cache->n_pages * cache->n_kv_head > 0x7fffffff) return LR_E_UNSUPPORTED;
   const int64_t most = (int64_t)batch->pages * cache->page;
   if (batch->B > 65535 || most > (1 << 30) || batch->B * (most / 32 + 8) >= 0x7fffffff) return LR_E_UNSUPPORTED;
   c.k = (u8*)cache->k;

@@ -71,7 +71,7 @@ def calls(hip, cache, batch, which=(WRITE, READ, ATTEND), rows=5, Hq=8, ld=None,
     (dict(n_pages=0), E_SHAPE), (dict(n_kv_head=0), E_SHAPE), (dict(page=0), E_SHAPE), (dict(head_dim=-64), E_SHAPE), (dict(B=0), E_SHAPE),
     (dict(pages=0), E_SHAPE), (dict(ld_table=3), E_SHAPE), (dict(n_kv_head=3), E_SHAPE),
     (dict(page=8), E_UNSUPPORTED), (dict(page=24), E_UNSUPPORTED), (dict(page=512), E_UNSUPPORTED), (dict(head_dim=96), E_UNSUPPORTED),
-    (dict(head_dim=256), E_UNSUPPORTED), (dict(format=2), E_UNSUPPORTED), (dict(B=65536), E_UNSUPPORTED),
+    (dict(head_dim=256), E_UNSUPPORTED), (dict(format=2), E_UNSUPPORTED), (dict(B=65536), E_UNSUPPORTED), (dict(n_pages=1 << 30), E_UNSUPPORTED),
     (dict(page=256, pages=(1 << 22) + 1, ld_table=1 << 23), E_UNSUPPORTED),
     (dict(starts=None), E_SHAPE),      # one row per sequence: 3, not 5
 ])
