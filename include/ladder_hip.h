@@ -796,7 +796,7 @@ int lr_linear_multi_route(const lr_projection_t* projections, int n_projections,
  * A cache holds k and v, [n_pages, n_kv_head, page, head_dim], in bf16 or e4m3 (float8_e4m3fn).  An e4m3 row is x / 2^e rounded
  * once, e the smallest exponent with max|x| <= 448 * 2^e over the row's finite values (at least -126; what is not finite is NaN);
  * scales [n_pages, n_kv_head, 2, page] holds e + 127 as a byte, those of a page's keys, then those of its values.  What is
- * read back is exact in bf16.  page: a power of two from 16 to 256; head_dim 64 or 128 (LR_E_UNSUPPORTED otherwise).
+ * read back is exact in bf16.  page: a power of two from 16 to 256; head_dim 64 or 128; n_pages * n_kv_head below 2^31 (LR_E_UNSUPPORTED otherwise).
  *
  * A batch is B sequences: table [B, pages] (row stride ld_table) names their pages in order, lengths [B] how many tokens they have,
  * the call's own among them.  starts [B + 1], ascending from 0: the call's rows starts[b] .. starts[b + 1] - 1 are the last tokens of
