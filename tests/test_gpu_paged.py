@@ -60,6 +60,8 @@ def written(case, hq, rope, rot, interleaved, qkv, dtype=F32):
     (14, 2, 64, 256, 16, BF, [300, 2], [299, 2]),
     (2, 1, 128, 64, None, BF, [70, 64], [70, 1]),                        # nothing turned
     (16, 8, 128, 128, 64, F32, [129] + [3] * 69, None),                  # more sequences than a wave has lanes
+    (2, 1, 64, 64, 48, F32, [1500, 700, 1103], [1500, 0, 1101]),         # workgroups of several tokens
+    (1, 1, 128, 16, 128, BF, [1300, 30], [1290, 30]),
 ])
 def test_write(hip, e4m3, interleaved, hq, hkv, hd, page, rot, table, lengths, new):
     case = Case(lengths, hkv, hd, page, e4m3, seed=3, new=new)
@@ -192,7 +194,7 @@ def test_rows_and_pages_out_of_range_are_left_alone(hip):
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("hkv,hd,page,lengths,new", [
     (1, 128, 16, [1], None), (2, 64, 32, [33, 0, 32, 5], None), (8, 128, 64, [130, 64, 1], [130, 64, 1]), (3, 64, 16, [50, 7], [20, 0]),
-    (1, 64, 256, [1] * 130, [1] * 130), (24, 128, 128, [300], [300]),
+    (1, 64, 256, [1] * 130, [1] * 130), (24, 128, 128, [300], [300]), (1, 64, 32, [1700, 3, 0, 1000], [1700, 2, 0, 999]),
 ])
 def test_read(hip, e4m3, hkv, hd, page, lengths, new):
     case = Case(lengths, hkv, hd, page, e4m3, seed=6, new=new)
