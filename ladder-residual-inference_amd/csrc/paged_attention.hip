@@ -114,8 +114,15 @@ struct PagedDecode {
 // What a sequence costs a worker besides its tiles, in tiles (7 us in a row of short sequences for two of them; a tile 0.45 us): as much more room
 // it has on the line.
 constexpr int PAGED_SEQUENCE = 6;
-// A sequence's parts are put together by the last of its workers, of no more than so many at a time: more go through their blocks' last ones.
-constexpr int PAGED_BLOCK = 16;
+// A sequence's parts are read that many at a time by the last of its workers; where there are more than PAGED_ONE, blocks of so many workers go first.  (us,
+// 24 sequences of up to 4096 keys with 32 workers per kv head: 26.4, all through blocks 27.8.)
+constexpr int PAGED_BLOCK = 16, PAGED_ONE = 32;
+// Parts of a sequence, where they would have fewer than PAGED_FEW tiles: 62 parts of 4 tiles take 15.0 us, 16 of 16 13.8 (16 q heads on one kv head of 128, 7888
+// keys); at 30000 235 parts of 4 17.0, 59 of 16 19.1.
+constexpr int PAGED_PARTS = 16, PAGED_FEW = 16;
+// Tiles of a worker that sequences cut on their own may cost.  us, the line / sequences: 7 of 7888 keys, 16 q heads on one kv head 26.6 / 15.9; 14 of up to 843,
+// 8 kv heads 17.1 / 10.4; 24 of up to 4096 with 16 instead of 8 27.4 / 27.9.
+constexpr int PAGED_MORE = 8;
 
 template <int HD, bool E4M3>
 __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4M3>::PER_CU * DecodeTile<HD, E4M3>::NW / 4)) void k_paged_decode(const PagedCache c, const PagedBatch t, const PagedDecode a) {
@@ -153,21 +160,47 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
       }
     }
   }
-  const int workers = min((int)gridDim.x, max((total + NW - 1) / NW, sequences)), w = blockIdx.x;   // (a tile for each wave, or a sequence)
-  if (w >= workers) return;
-  // what a sequence costs besides its tiles, as more room on the line: where workers have one sequence or several; where a sequence has
-  // many workers, it is the same for all of them
-  const int extra = 2 * sequences >= workers ? PAGED_SEQUENCE : 0;
-  total += extra * sequences;
-  auto places_upto = [&]() { return upto + extra * __popcll(some & (~0ull >> (63 - lane))); };   // of the 64 sequences, in all lanes
-  // equal parts, the first `larger` of them a tile more
-  const int each = (u32)total / (u32)workers, larger = total - each * workers;
-  int at = w * each + min(w, larger);
-  const int end = at + each + (w < larger);
-  // the sequence that `at` belongs to: b0 + s, which begins at `first`
-  int s, first;
-  {
+  // a worker's tiles at least: one for each of its waves, and where that leaves a sequence no more than PAGED_PARTS parts up to PAGED_FEW
+  const auto few = [&](int tiles) { return tiles <= PAGED_PARTS * PAGED_FEW ? max(NW, (tiles + PAGED_PARTS - 1) / PAGED_PARTS) : NW; };
+  const int w = blockIdx.x;
+  int workers = min((int)gridDim.x, max((total + NW - 1) / NW, sequences));
+  if (sequences == 1 && few(total) > NW) workers = min(workers, PAGED_PARTS);
+  // Workers from0 on take equal parts of the line from `line0` on, `each` places and the first `larger` of them one more; this one's begins in sequence
+  // b0 + s, which begins at `first`
+  int from0 = 0, line0 = 0, each = 0, larger, s, first, extra = 0;
+  // Sequences cut on their own, into equal parts of no more than `most` tiles, where that takes few tiles more than the line in equal parts: a worker has
+  // one sequence only, and its results to join with others' once.
+  if (t.B <= 64 && sequences > 1 && sequences < workers) {
+    const int even = max((total + workers - 1) / workers, few(wave_max(tiles))), last = even + PAGED_MORE;
+    // (half a part per sequence is lost: hopeless where even the last does not have that much room)
+    for (int most = (long long)last * ((int)gridDim.x - sequences / 2) < total ? last + 1 : even; most <= last; most += 1 + most / 8) {
+      const int parts = (u32)(tiles + most - 1) / (u32)most, sum = paged_sums(parts), all = __builtin_amdgcn_readlane(sum, 63);
+      if (all > (int)gridDim.x) continue;
+      if (w >= all) return;
+      s = __popcll(__ballot(sum <= w)) & 63;
+      const int n = __builtin_amdgcn_readlane(parts, s), mine = __builtin_amdgcn_readlane(tiles, s);
+      from0 = __builtin_amdgcn_readlane(sum, s) - n;
+      line0 = first = __builtin_amdgcn_readlane(upto, s) - mine;
+      each = (u32)mine / (u32)n;
+      larger = mine - each * n;
+      break;
+    }
+  }
+  const bool alone = each > 0;
+  if (!alone) {
+    if (w >= workers) return;
+    // what a sequence costs besides its tiles, as more room on the line: where workers have one sequence or several; where a sequence has
+    // many workers, it is the same for all of them
+    extra = 2 * sequences >= workers ? PAGED_SEQUENCE : 0;
+    total += extra * sequences;
+    each = (u32)total / (u32)workers;
+    larger = total - each * workers;
+  }
+  int at = line0 + (w - from0) * each + min(w - from0, larger);
+  const int end = at + each + (w - from0 < larger);
+  if (!alone) {
     int before = 0;
+    auto places_upto = [&]() { return upto + extra * __popcll(some & (~0ull >> (63 - lane))); };   // of the 64 sequences, in all lanes
     if (t.B > 64) {
       for (int i = 0;; i += 64) {
         look(i);
@@ -513,14 +546,14 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
     for (int ks = 0; ks < KS; ++ks) qf[ks] = qn[ks];
   }
 
-  // ---- parts put together (at the end: the stream above waits for nobody).  Workers w0 .. w1 have parts of a sequence; those of one block of
-  // PAGED_BLOCK workers are put together by the block's last, the blocks' results by the last block's.
+  // ---- parts put together (at the end: the stream above waits for nobody).  Workers w0 .. w1 have parts of a sequence, which the last of them puts
+  // together; where they are more than PAGED_ONE, those of a block of PAGED_BLOCK workers by the block's last, and the blocks' results by the last block's.
   const int n_blocks = (gridDim.x + PAGED_BLOCK - 1) / PAGED_BLOCK, kw = w / PAGED_BLOCK, block_parts = 2 * (int)(gridDim.y * gridDim.x);
-  const auto worker = [&](int place) {
-    const int n = larger * (each + 1);
-    return (int)(place < n ? (u32)place / (u32)(each + 1) : larger + (u32)(place - n) / (u32)each);
+  const auto worker = [&](int at) {
+    const int place = at - line0, n = larger * (each + 1);
+    return from0 + (int)(place < n ? (u32)place / (u32)(each + 1) : larger + (u32)(place - n) / (u32)each);
   };
-  // workers' parts first (of a block, or all of them where they are one block's), then blocks'; part u lies at places + 2 u, + 1 for the one
+  // workers' parts first (of a block, or all of them), then blocks'; part u lies at places + 2 u, + 1 for the one
   // with the sequence's first tile
   struct Open {
     u32* ticket;
@@ -533,7 +566,8 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
     const int w0 = worker(open_first[i]), w1 = worker(open_first[i] + open_tiles[i] - 1);
     k0[i] = w0 / PAGED_BLOCK;
     k1[i] = w1 / PAGED_BLOCK;
-    const bool one = k0[i] == k1[i];
+    const bool one = k0[i] == k1[i] || w1 - w0 < PAGED_ONE;
+    if (one) k1[i] = k0[i];
     p.u0 = one ? w0 : max(w0, kw * PAGED_BLOCK);
     p.u1 = one ? w1 : min(w1, kw * PAGED_BLOCK + PAGED_BLOCK - 1);
     p.places = group * (int)gridDim.x * 2;

@@ -245,6 +245,7 @@ def test_decode(hip, e4m3, hq, hkv, hd, page, lengths):
 @pytest.mark.parametrize("lengths,hq,hkv,hd,page", [
     ([9001], 4, 1, 128, 16), ([5000, 1, 0, 700], 2, 2, 64, 32), ([33] * 300, 2, 1, 64, 16), ([0] * 70 + [100], 4, 4, 128, 64),
     ([2049, 4095], 8, 1, 128, 128), ([0, 0], 8, 1, 128, 16),
+    ([20000, 300, 0, 9000], 2, 1, 128, 64), ([700] * 5 + [3], 20, 1, 64, 16), ([1500, 3, 40, 900] * 7, 8, 8, 64, 32), ([26000], 17, 1, 128, 256),
 ])
 def test_decode_of_long_and_of_many_sequences(hip, e4m3, lengths, hq, hkv, hd, page):
     attend(Case(lengths, hkv, hd, page, e4m3, seed=5), hq)
