@@ -18,8 +18,8 @@ struct PagedQuery {
 
 // ------------------------------------------------------------------------------------ one row per sequence
 // All sequences' keys lie on one line of tiles of 32, sequence after sequence, and the workers of a kv head (workgroups of four waves) take
-// equal parts of it, wherever sequences begin and end: batches of any lengths keep the chip evenly busy, and the host, which knows no
-// length, launches the same grid always.  A part of a sequence leaves its maximum, sum and weighted values in the scratch, and whoever ends
+// equal parts of it, wherever sequences begin and end (or of each sequence, where these are few): batches of any lengths keep the chip evenly busy,
+// and the host, which knows no length, launches the same grid always.  A part of a sequence leaves its maximum, sum and weighted values in the scratch, and whoever ends
 // last puts a sequence's parts together (in their order: the same bits every time); a sequence inside one part is written directly.
 //
 // A wave streams tiles of its own through its own LDS (no barrier in the loop): rows come by loads straight into LDS, K's of the next tile
@@ -29,7 +29,7 @@ struct PagedQuery {
 // weight).  e4m3: K is expanded with its row's power of two on the way to the product, V without, its power goes into the weight.
 //
 // Bound: memory.  64 sequences of 2048 keys, 8 kv heads of 128, e4m3: 43.4 us, 6.3 TB/s (a plain read 7.0); one of 131072 in bf16 85.5 us, 6.3 TB/s;
-// 24 of 1 to 4096 27.4 us.  One workgroup per CU with four waves whose tiles are all in flight reads faster than two or three smaller ones (the first
+// 24 of 1 to 4096 26.6 us.  One workgroup per CU with four waves whose tiles are all in flight reads faster than two or three smaller ones (the first
 // of these 43.6, 50, 58), rows that nobody else reads come non-temporally (10 %).  Few keys: a chain of waits, 8.4 us for one sequence of 2048
 // and one kv head: the lengths 0.7, page numbers and q 1.1, keys, values and products 1.5, four waves' results 0.9, what a worker leaves
 // and its ticket 1.0, the parts together 1.8, the rest the launch.
