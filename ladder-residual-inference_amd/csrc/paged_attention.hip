@@ -706,7 +706,12 @@ static int launch_paged_decode(const PagedCache& c, const PagedBatch& t, const P
 // the first portion, the rows stored; 6.7 us) 109.  Slower: products and exponentials of two tiles interleaved (137 -> 140), two groups of waves in
 // turn (26.8 -> 28.4 for the 256 tokens behind 8000 that take 26.5), workgroups that take several blocks (the registers spill: 138 -> 146).
 constexpr int PROMPT_ROWS = 128, PROMPT_KEYS = 64;
-constexpr int PROMPT_SPLIT_KEYS = 256;   // a part of a row's keys has at least so many
+// Into how many parts a row's keys are cut at most: of 128 up to 16 parts, which are joined at once, else of 256.  (us, all of 256 / this: 4 sequences of 420 and 4
+// tokens of the 8B model 14.1 / 10.6, 23 behind 1057 15.7 / 13.5; all of 128 / this: 8 tokens of 8 q heads on one kv head behind 7000 17.5 / 15.9.)
+__host__ __device__ constexpr int prompt_parts_of(int keys) {
+  const int half = (keys + 127) / 128, whole = (keys + 255) / 256;
+  return half <= 16 ? half : whole > 16 ? whole : 16;
+}
 
 struct PagedPrompt {
   const u16* q;
@@ -762,7 +767,7 @@ __device__ __forceinline__ int prompt_keys(const PromptBlock& at, int G) {
   return max(0, at.ahead + last / G + 1);
 }
 // and into how many parts they are cut
-__device__ __forceinline__ int prompt_parts(int keys, int n_split) { return max(1, min(n_split, (keys + PROMPT_SPLIT_KEYS - 1) / PROMPT_SPLIT_KEYS)); }
+__device__ __forceinline__ int prompt_parts(int keys, int n_split) { return max(1, min(n_split, prompt_parts_of(keys))); }
 
 template <int HD, int KSP>
 struct PromptLds {
@@ -1240,7 +1245,7 @@ static PromptPlan prompt_plan(const PagedCache& c, const PagedBatch& t, int hd, 
   p.items = ((int64_t)rows * G + (PROMPT_ROWS - 1) * some) / PROMPT_ROWS;
   p.bound = p.items > 0x3fffffff ? 0x3fffffff : (int)p.items;
   p.items *= c.Hkv;
-  const int64_t most = (((int64_t)t.pages << c.shift) + PROMPT_SPLIT_KEYS - 1) / PROMPT_SPLIT_KEYS;
+  const int most = prompt_parts_of(t.pages << c.shift);
   int64_t n = p.items ? cus / p.items : 1;
   if (n > most) n = most;
   // Parts save a row's last block (1 - 1 / n) of its portions, about 1.3 us each, and cost a second launch, 4 to 6 us.  us, one part / several:
