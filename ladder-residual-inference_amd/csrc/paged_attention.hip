@@ -30,8 +30,8 @@ struct PagedQuery {
 //
 // Bound: memory.  64 sequences of 2048 keys, 8 kv heads of 128, e4m3: 43.4 us, 6.3 TB/s (a plain read 7.0); one of 131072 in bf16 85.5 us, 6.3 TB/s;
 // 24 of 1 to 4096 26.6 us.  One workgroup per CU with four waves whose tiles are all in flight reads faster than two or three smaller ones (the first
-// of these 43.6, 50, 58), rows that nobody else reads come non-temporally (10 %).  Few keys: a chain of waits, 8.4 us for one sequence of 2048
-// and one kv head: the lengths 0.7, page numbers and q 1.1, keys, values and products 1.5, four waves' results 0.9, what a worker leaves
+// of these 43.6, 50, 58), rows that nobody else reads come non-temporally (10 %).  Few keys: a chain of waits, 8.4 us at first for one sequence of 2048
+// and one kv head, 7.3 now: the lengths 0.7, page numbers and q 1.1, keys, values and products 1.5, four waves' results 0.9, what a worker leaves
 // and its ticket 1.0, the parts together 1.8, the rest the launch.
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x2_t __attribute__((ext_vector_type(2)));
@@ -123,11 +123,17 @@ constexpr int PAGED_PARTS = 16, PAGED_FEW = 16;
 // Tiles of a worker that sequences cut on their own may cost.  us, the line / sequences: 7 of 7888 keys, 16 q heads on one kv head 26.6 / 15.9; 14 of up to 843,
 // 8 kv heads 17.1 / 10.4; 24 of up to 4096 with 16 instead of 8 27.4 / 27.9.
 constexpr int PAGED_MORE = 8;
+// Tiles of sequences that are not cut at all where there are many.  us, cut / whole: 40 of up to 270 keys, 8 kv heads of 64 10.9 / 7.6; 46 of up to 478, of 128
+// 15.4 / 11.2; of 34 of up to 300, 24 kv heads 21.0 / 15.5.
+constexpr int PAGED_WHOLE = 16;
 
-template <int HD, bool E4M3>
+// MANY: more than one place in the batch.  (A kernel of its own for one: less to look up, and no scalar registers kept in lanes of vector ones;
+// 8.4 -> 7.3 us for 2048 keys of one kv head.)
+template <int HD, bool E4M3, bool MANY>
 __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4M3>::PER_CU * DecodeTile<HD, E4M3>::NW / 4)) void k_paged_decode(const PagedCache c, const PagedBatch t, const PagedDecode a) {
   using T = DecodeTile<HD, E4M3>;
   constexpr int KS = HD / 32, DT = HD / 16, NW = T::NW;   // k-steps of a score product; 16-dimension tiles of O^T
+  const int B = MANY ? t.B : 1;
   extern __shared__ __attribute__((aligned(1024))) unsigned char paged_lds[];
   float (*const s_ml)[16][2] = reinterpret_cast<float (*)[16][2]>(paged_lds + NW * (T::WAVE + T::RESULT));   // [NW]
   u32* const s_ticket = reinterpret_cast<u32*>(paged_lds + NW * (T::WAVE + T::RESULT + 128));
@@ -142,18 +148,18 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
   unsigned long long some;   // which of them have tiles
   auto look = [&](int from) {
     b0 = from;
-    len = b0 + lane < t.B ? paged_length(t, c.shift, b0 + lane) : 0;
+    len = b0 + lane < B ? paged_length(t, c.shift, b0 + lane) : 0;
     tiles = (len + 31) >> 5;
     upto = paged_sums(tiles);
     some = __ballot(tiles > 0);
   };
   int total = 0, sequences = 0;
-  for (int i = 0; i < t.B; i += 64) {
+  for (int i = 0; i < B; i += 64) {
     look(i);
     total += __builtin_amdgcn_readlane(upto, 63);
     sequences += __popcll(some);
     if (wave == 0) {   // empty places: zeros, one worker each
-      unsigned long long empty = __ballot(i + lane < t.B && tiles == 0 && (i + lane) % gridDim.x == blockIdx.x);
+      unsigned long long empty = __ballot(i + lane < B && tiles == 0 && (i + lane) % gridDim.x == blockIdx.x);
       for (; empty; empty &= empty - 1) {
         u16* const y = a.y + (int64_t)(i + __builtin_ctzll(empty)) * a.ldy + h0 * HD;
         for (int d = lane * 8; d < nh * HD; d += 512) st16(y + d, make_uint4(0, 0, 0, 0));
@@ -170,8 +176,9 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
   int from0 = 0, line0 = 0, each = 0, larger, s, first, extra = 0;
   // Sequences cut on their own, into equal parts of no more than `most` tiles, where that takes few tiles more than the line in equal parts: a worker has
   // one sequence only, and its results to join with others' once.
-  if (t.B <= 64 && sequences > 1 && sequences < workers) {
-    const int even = max((total + workers - 1) / workers, few(wave_max(tiles))), last = even + PAGED_MORE;
+  const int longest = MANY && B <= 64 && sequences > 1 ? wave_max(tiles) : 0;   // (0: not known or not wanted)
+  if (longest && sequences < workers) {
+    const int even = max((total + workers - 1) / workers, few(longest)), last = even + PAGED_MORE;
     // (half a part per sequence is lost: hopeless where even the last does not have that much room)
     for (int most = (long long)last * ((int)gridDim.x - sequences / 2) < total ? last + 1 : even; most <= last; most += 1 + most / 8) {
       const int parts = (u32)(tiles + most - 1) / (u32)most, sum = paged_sums(parts), all = __builtin_amdgcn_readlane(sum, 63);
@@ -197,19 +204,27 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
     larger = total - each * workers;
   }
   int at = line0 + (w - from0) * each + min(w - from0, larger);
-  const int end = at + each + (w - from0 < larger);
+  int end = at + each + (w - from0 < larger);
   if (!alone) {
     int before = 0;
     auto places_upto = [&]() { return upto + extra * __popcll(some & (~0ull >> (63 - lane))); };   // of the 64 sequences, in all lanes
-    if (t.B > 64) {
+    if (B > 64) {
       for (int i = 0;; i += 64) {
         look(i);
         const int n = __builtin_amdgcn_readlane(upto, 63) + extra * __popcll(some);
-        if (at < before + n || i + 64 >= t.B) break;
+        if (at < before + n || i + 64 >= B) break;
         before += n;
       }
     }
     const int places = places_upto();
+    if (longest && longest <= PAGED_WHOLE) {   // short sequences go whole to the worker that has their middle: nothing to join
+      const int middle = places - (tiles + extra) / 2;
+      const unsigned long long from = __ballot(tiles > 0 && middle >= at), behind = __ballot(tiles > 0 && middle >= end);
+      if (from == behind) return;
+      const auto begin = [&](int i) { return __builtin_amdgcn_readlane(places, i) - __builtin_amdgcn_readlane(tiles, i) - extra; };
+      at = begin(__builtin_ctzll(from));
+      end = behind ? begin(__builtin_ctzll(behind)) : total;
+    }
     s = __popcll(__ballot(before + places <= at)) & 63;
     first = before + __builtin_amdgcn_readlane(places, s) - __builtin_amdgcn_readlane(tiles, s) - extra;
   }
@@ -236,11 +251,12 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
   };
   // on to the next sequence that has tiles; false: this worker's part of the line ends before its first one
   auto next_segment = [&](Segment& g) {
+    if constexpr (!MANY) return false;
     first += __builtin_amdgcn_readlane(tiles, s) + extra;
     if (first + extra >= end) return false;
     unsigned long long others = some & (s == 63 ? 0ull : ~0ull << (s + 1));
     while (!others) {
-      if (b0 + 64 >= t.B) return false;
+      if (b0 + 64 >= B) return false;
       look(b0 + 64);
       others = some;
     }
@@ -310,7 +326,10 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
     if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2_t, f32x2_t{M, L}), mres, (part * 16 + h) * 8, 0, PAGED_COHERENT);
   };
   // the sequences of which others have parts, too: one that began before this worker, one that goes on behind it
-  int open_b[2] = {-1, -1}, open_first[2], open_tiles[2];
+  constexpr int OPEN = MANY ? 2 : 1;
+  int open_b[OPEN], open_first[OPEN] = {}, open_tiles[OPEN] = {};
+#pragma unroll
+  for (int i = 0; i < OPEN; ++i) open_b[i] = -1;
   Segment g = segment();
   if (g.to <= g.from && !next_segment(g)) return;   // (the sequence's cost alone)
   bf16x8_t qf[KS];
@@ -534,7 +553,7 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
       else store_part(slot, h, d, v, M, L);
     }
     if (!whole) {
-      const int i = g.from == 0;
+      const int i = MANY && g.from == 0;
       open_b[i] = g.b;
       open_first[i] = g.first;
       open_tiles[i] = g.n_tiles;
@@ -559,7 +578,7 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
     u32* ticket;
     int u0, u1, places, began, n_parts;
   };
-  int k0[2] = {}, k1[2] = {};
+  int k0[OPEN] = {}, k1[OPEN] = {};
   auto workers_of = [&](int i) {
     Open p = {};
     if (open_b[i] < 0) return p;
@@ -572,7 +591,7 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
     p.u1 = one ? w1 : min(w1, kw * PAGED_BLOCK + PAGED_BLOCK - 1);
     p.places = group * (int)gridDim.x * 2;
     p.began = w0;
-    p.ticket = a.tickets + (one ? (int64_t)group * t.B + open_b[i] : (int64_t)gridDim.y * t.B + (group * n_blocks + kw) * 2 + (kw == k0[i]));
+    p.ticket = a.tickets + (one ? (int64_t)group * B + open_b[i] : (int64_t)gridDim.y * B + (group * n_blocks + kw) * 2 + (kw == k0[i]));
     p.n_parts = p.u1 - p.u0 + 1;
     return p;
   };
@@ -584,20 +603,22 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
       s_ticket[i] = was + 1;
     }
   };
-  if (open_b[0] < 0 && open_b[1] < 0) return;
-  Open both[2] = {workers_of(0), workers_of(1)};
+  if (open_b[0] < 0 && open_b[OPEN - 1] < 0) return;
+  Open both[OPEN];
+#pragma unroll
+  for (int i = 0; i < OPEN; ++i) both[i] = workers_of(i);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   barrier();
-  count(both[0], 0);
-  count(both[1], 1);
+#pragma unroll
+  for (int i = 0; i < OPEN; ++i) count(both[i], i);
   barrier();
-  const bool last0 = both[0].n_parts && s_ticket[0] == (u32)both[0].n_parts, last1 = both[1].n_parts && s_ticket[1] == (u32)both[1].n_parts;
+  const bool last0 = both[0].n_parts && s_ticket[0] == (u32)both[0].n_parts, last1 = MANY && both[OPEN - 1].n_parts && s_ticket[1] == (u32)both[OPEN - 1].n_parts;
   asm volatile("" ::: "memory");
 #pragma unroll 1
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < OPEN; ++i) {
     bool last = i ? last1 : last0;
-    Open p = i ? both[1] : both[0];
-    const int b = i ? open_b[1] : open_b[0], first_block = i ? k0[1] : k0[0], last_block = i ? k1[1] : k1[0];
+    Open p = i ? both[OPEN - 1] : both[0];
+    const int b = i ? open_b[OPEN - 1] : open_b[0], first_block = i ? k0[OPEN - 1] : k0[0], last_block = i ? k1[OPEN - 1] : k1[0];
     bool final = first_block == last_block;
     const int block = (group * n_blocks + kw) * 2 + (kw == first_block ? 1 : 0);
 #pragma unroll 1
@@ -640,7 +661,7 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
       }
       if (final) break;
       final = true;
-      p = {a.tickets + (int64_t)group * t.B + b, first_block, last_block, block_parts + group * n_blocks * 2, first_block, last_block - first_block + 1};
+      p = {a.tickets + (int64_t)group * B + b, first_block, last_block, block_parts + group * n_blocks * 2, first_block, last_block - first_block + 1};
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       barrier();
       count(p, 0);
@@ -683,10 +704,13 @@ static int launch_paged_decode(const PagedCache& c, const PagedBatch& t, const P
   a.o_part = (float*)((u8*)scratch + p.ticket_bytes);
   a.ml_part = (float*)((u8*)a.o_part + p.o_bytes);
   constexpr size_t lds = DecodeTile<HD, E4M3>::LDS;
-  static std::atomic<unsigned long long> raised{0};
-  if (!lr_raise_lds_limit(reinterpret_cast<const void*>(&k_paged_decode<HD, E4M3>), lds, raised)) return LR_E_LAUNCH;
-  k_paged_decode<HD, E4M3><<<dim3(p.workers, p.groups), dim3(64 * DecodeTile<HD, E4M3>::NW), lds, s>>>(c, t, a);
-  return lr_launch_status();
+  static std::atomic<unsigned long long> raised[2] = {};
+  const auto as = [&](auto MANY) -> int {
+    if (!lr_raise_lds_limit(reinterpret_cast<const void*>(&k_paged_decode<HD, E4M3, MANY>), lds, raised[MANY])) return LR_E_LAUNCH;
+    k_paged_decode<HD, E4M3, MANY><<<dim3(p.workers, p.groups), dim3(64 * DecodeTile<HD, E4M3>::NW), lds, s>>>(c, t, a);
+    return lr_launch_status();
+  };
+  return t.B > 1 ? as(std::true_type{}) : as(std::false_type{});
 }
 
 // ------------------------------------------------------------------------------------ rows of prompts
