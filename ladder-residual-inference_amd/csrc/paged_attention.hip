@@ -198,7 +198,7 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
     if (w >= workers) return;
     // what a sequence costs besides its tiles, as more room on the line: where workers have one sequence or several; where a sequence has
     // many workers, it is the same for all of them
-    extra = 2 * sequences >= workers ? PAGED_SEQUENCE : 0;
+    extra = MANY && 2 * sequences >= workers ? PAGED_SEQUENCE : 0;
     total += extra * sequences;
     each = (u32)total / (u32)workers;
     larger = total - each * workers;
@@ -582,7 +582,7 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
   auto workers_of = [&](int i) {
     Open p = {};
     if (open_b[i] < 0) return p;
-    const int w0 = worker(open_first[i]), w1 = worker(open_first[i] + open_tiles[i] - 1);
+    const int w0 = MANY ? worker(open_first[i]) : 0, w1 = MANY ? worker(open_first[i] + open_tiles[i] - 1) : workers - 1;
     k0[i] = w0 / PAGED_BLOCK;
     k1[i] = w1 / PAGED_BLOCK;
     const bool one = k0[i] == k1[i] || w1 - w0 < PAGED_ONE;

@@ -251,6 +251,14 @@ def test_decode_of_long_and_of_many_sequences(hip, e4m3, lengths, hq, hkv, hd, p
     attend(Case(lengths, hkv, hd, page, e4m3, seed=5), hq)
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 1, 128), (12, 4, 64), (17, 1, 128)])
+def test_decode_of_one_sequence(hip, e4m3, hq, hkv, hd):
+    """Around a tile, a tile for each wave, two workers, and from single tiles of a worker's waves to several."""
+    for n in (0, 1, 32, 33, 96, 128, 129, 160, 161, 200, 255, 256, 257, 300, 511, 513, 2047, 2049, 2100, 4000, 8192, 8193, 8300):
+        attend(Case([n], hkv, hd, 64, e4m3, seed=n), hq)
+
+
 PROMPT = 2.0 ** -8      # prompts: a weight enters as one bf16 number
 
 
