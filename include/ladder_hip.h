@@ -855,7 +855,7 @@ int lr_paged_read(const lr_paged_read_t* desc, lr_stream_t stream);
  * Hq / n_kv_head; q, y [rows, Hq head_dim] (row strides ldq, ldy) with no memory in common.  The cache holds the call's tokens already.
  * A row that sees no key is zeros; keys of a page out of range, and those behind the table's pages, count as not there; what keys that a
  * row does not see hold, NaN too, does not reach it.  Scores, softmax and sums in fp32; a weight enters the matrix cores as two bf16
- * numbers where starts is NULL, else as one; one rounding of y.  scale: positive, up to 2^64.
+ * numbers (2^-16 of it is lost), as in lr_attn_prefill; one rounding of y.  scale: positive, up to 2^64.
  * scratch: lr_paged_attention_scratch_bytes() (0: sizes that are refused), zero before the first call and kept for calls with the same
  * cache but for its addresses and n_pages, the same B, pages, Hq and starts or none (rows no more than those it was sized for), one
  * after the other: calls that may overlap have their own. */

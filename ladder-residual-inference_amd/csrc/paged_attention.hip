@@ -718,17 +718,18 @@ static int launch_paged_decode(const PagedCache& c, const PagedBatch& t, const P
 // a wave 32, whatever G is: the columns of the products
 //   S^T[key][row] = K q^T,   O^T[dim][row] += V^T P^T
 // on the matrix cores (32x32x16).  A column is a lane, so maxima, sums and factors are a lane's own, and the 16 scores that it holds of 32 keys are, in
-// their order, the second product's operand.  Weights enter as one bf16 number: y is off by their rounding, at most 2^-8 of each and at random,
-// where keys are many about as much as by y's own rounding (1.41 times the error of exact sums rounded).  Keys come 64 at a time into one of
+// their order, the second product's operand.  Weights enter as two bf16 numbers (2^-16 of the weight), as in a step of single tokens and in the prompts
+// of the contiguous cache: a third of the products, 173 us instead of 136 for the prompts below.  (One number loses up to 2^-8 of each weight, about as
+// much of y as its own rounding.)  Keys come 64 at a time into one of
 // two buffers, one barrier per 64; bf16 by loads straight into LDS, e4m3 through registers, expanded on the way with its row's power of two:
 // from there on the two are the same.
 // Few rows: a workgroup's keys are cut among several, whose results a second launch puts together.
 //
-// Bound: the waves' instructions, one after another: 32 products of 32 cycles, 32 exponentials of 16 and some 250 others of 4 or more per wave
+// Bound: the waves' instructions, one after another: 48 products of 32 cycles, 32 exponentials of 16 and some 300 others of 4 or more per wave
 // and 64 keys; two waves a SIMD (222 registers) hide little more of one another than this.  Five prompts of up to 2048 tokens, 32 q and 8 kv heads of
-// 128: 135 to 141 us, 0.82 PFLOP/s of the 1.35 of a large library product; without what a workgroup does once (its block looked up, q,
-// the first portion, the rows stored; 6.7 us) 109.  Slower: products and exponentials of two tiles interleaved (137 -> 140), two groups of waves in
-// turn (26.8 -> 28.4 for the 256 tokens behind 8000 that take 26.5), workgroups that take several blocks (the registers spill: 138 -> 146).
+// 128: 173 us (e4m3 186), 0.65 PFLOP/s of the 1.35 of a large library product, 0.98 with the weights' second numbers counted.  Slower, measured with
+// weights of one number: products and exponentials of two tiles interleaved (137 -> 140), two groups of waves in turn (26.8 -> 28.4 for 256 tokens behind
+// 8000), workgroups that take several blocks (the registers spill: 138 -> 146).
 constexpr int PROMPT_ROWS = 128, PROMPT_KEYS = 64;
 // Into how many parts a row's keys are cut at most: of 128 up to 16 parts, which are joined at once, else of 256.  (us, all of 256 / this: 4 sequences of 420 and 4
 // tokens of the 8B model 14.1 / 10.6, 23 behind 1057 15.7 / 13.5; all of 128 / this: 8 tokens of 8 q heads on one kv head behind 7000 17.5 / 15.9.)
@@ -1005,14 +1006,16 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
     m = mn;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      u32x4_t pw[2];
+      u32x4_t ph[2], pl[2];
 #pragma unroll
       for (int h2 = 0; h2 < 2; ++h2)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float x0 = exp2_hw(fmaf(sacc[n][8 * h2 + 2 * j], c2, nmc)), x1 = exp2_hw(fmaf(sacc[n][8 * h2 + 2 * j + 1], c2, nmc));   // masked: 0
-          l += x0 + x1;   // (v_dot2_f32_bf16 on the rounded pair would be one instruction: the compiler reads the vector's first element for all four)
-          pw[h2][j] = pack_bf2(x0, x1);
+          l += x0 + x1;
+          const u32 hi = pack_bf2(x0, x1);
+          ph[h2][j] = hi;
+          pl[h2][j] = pack_bf2(x0 - bf_lo(hi), x1 - bf_hi(hi));
         }
       // k-step h2 covers keys 16 h2 + {0..3, 8..11} + 4 half of the tile, in the order of sacc
 #pragma unroll
@@ -1027,7 +1030,10 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[d], __builtin_bit_cast(bf16x8_t, pw[h2]), o[d], 0, 0, 0);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[d], __builtin_bit_cast(bf16x8_t, ph[h2]), o[d], 0, 0, 0);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[d], __builtin_bit_cast(bf16x8_t, pl[h2]), o[d], 0, 0, 0);
       }
     }
   };
@@ -1069,9 +1075,9 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
     if constexpr (E4M3)
       if (more) expand(buf ^ 1);
   }
-  // The products take a tile's values for all rows: one that is not finite reached also those that do not see its key, as 0 * v.  Rare, and
-  // not worth a look at every value: a wave that ends with something that is not finite, and has such a value among the keys that
-  // not all of its rows see, does its rows again, key by key.
+  // The products take a tile's values for all rows: one that is not finite reached also those that do not see its key, as 0 * v.  And an infinite
+  // one that all see met the weights' second numbers, of which some are zero or negative.  Rare, and not worth a look at every value: a wave that ends with
+  // something that is not finite, and has such a value among its keys, does its rows again, key by key.  (NaN that all rows see is right as it is.)
   {
     float none = 0.0f;
 #pragma unroll
@@ -1100,12 +1106,18 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
         return f32x4_t{bf_lo(x.x), bf_hi(x.x), bf_lo(x.y), bf_hi(x.y)};
       };
       bool some = false;
+      const auto finite = [](float x) { return fabsf(x) < INFINITY; };
+      constexpr int AT_ONCE = 64 / (HD / 8);   // keys: a lane looks at eight elements
 #pragma unroll 1
-      for (int key = max(0, pmin + 1); key < pmax + PROMPT_KEYS; ++key) {   // (those of its last portion that none of them sees, too)
-        const int page = my_key(key) ? page_of(key) : -1;
+      for (int k0 = t_first; k0 < t_end && k0 < pmax + PROMPT_KEYS; k0 += AT_ONCE) {   // (those of its last portion that none of them sees, too)
+        const int key = k0 + lane / (HD / 8), page = my_key(key) ? page_of(key) : -1;
         if (page < 0) continue;
-        const f32x4_t v = four(true, page, key, lane * 4 % HD);
-        some |= !(fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY);
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          const f32x4_t v = four(true, page, key, lane % (HD / 8) * 8 + j);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) some |= key > pmin ? !finite(v[e]) : fabsf(v[e]) == INFINITY;
+        }
       }
       if (__any(some)) {
 #pragma unroll

@@ -667,3 +667,53 @@ def test_refusals(hip):
         cache.batch(batch.table, batch.lengths, 5)
     with pytest.raises(AssertionError):
         cache.batch(batch.table.long(), batch.lengths, 4)
+
+
+# ------------------------------------------------------------------------------------------------ precision
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("hq,hkv,hd,page,lengths,new", [
+    (4, 1, 128, 16, [90, 33], [90, 33]), (2, 2, 64, 32, [200, 65], [70, 65]),        # four waves
+    (12, 1, 64, 64, [700], [700]), (2, 2, 128, 16, [640, 130], [400, 1]),            # eight
+    (8, 1, 128, 32, [3000], [65]), (4, 1, 64, 16, [2500, 700], [9, 40]),             # parts joined
+])
+def test_prompts_weights_have_two_numbers(hip, e4m3, hq, hkv, hd, page, lengths, new):
+    """A weight enters the matrix cores with 2^-16 of it lost, as in decode and as in lr_attn_prefill: one bf16 number would lose 2^-8."""
+    attend(Case(lengths, hkv, hd, page, e4m3, seed=51, new=new), hq, weight=WEIGHT)
+
+
+def test_both_caches_prompts_are_as_precise(hip):
+    """lr_attn_prefill on dense keys and the paged operator on the same ones, both within what two bf16 numbers per weight explain."""
+    hq, hkv, hd, n = 8, 2, 128, 150
+    case = Case([n], hkv, hd, 32, False, new=[n])
+    cache, batch, q, _ = attend(case, hq, weight=WEIGHT)
+    k, v = (torch.empty(n, hkv * hd, dtype=BF, device=DEV) for _ in range(2))
+    cache.read(batch, k, v)
+    kc, vc = (torch.zeros(1, hkv, 160, hd, dtype=BF, device=DEV) for _ in range(2))
+    kc[0, :, :n], vc[0, :, :n] = k.view(n, hkv, hd).transpose(0, 1), v.view(n, hkv, hd).transpose(0, 1)
+    qkv = torch.zeros(n, (hq + 2 * hkv) * hd, dtype=BF, device=DEV)
+    qkv[:, :hq * hd] = q.to(DEV)
+    y = torch.empty(n, hq * hd, dtype=BF, device=DEV)
+    hip.attn_prefill(qkv, kc, vc, torch.arange(n, dtype=torch.int32, device=DEV), y, 1, n, hq, hkv, hd)
+    want, spread, size = case.oracle(q, hq)
+    assert ((y.cpu().double().view(want.shape) - want).abs() <= bound(want, spread, size, n, hd, WEIGHT)).all()
+
+
+@pytest.mark.parametrize("lengths,new,hq,hkv", [([90], [20], 4, 1), ([700], [300], 4, 2), ([3000], [40], 8, 1), ([700], [700], 12, 1)])
+def test_infinite_values_go_through_prompts(hip, lengths, new, hq, hkv):
+    """An infinite value that all of a call's rows see, or some of them: infinite for those, nothing to the others, the other dimensions as they are."""
+    n, first = lengths[0], lengths[0] - new[0]
+    for at in (0, 37, first, first + new[0] // 2, n - 1):
+        case = Case(lengths, hkv, 64, 16, False, seed=52, new=new)
+        q = rnd(case.rows, hq * 64, seed=53)
+        want, spread, size = case.oracle(q, hq)
+        page, slot = int(case.table[0, at // 16]), at % 16
+        case.v[page, :, slot, 7], case.v[page, :, slot, 9] = math.inf, -math.inf
+        cache, batch = case.on(DEV, hq)
+        y = cache.attend(batch, q.to(DEV), torch.empty(case.rows, hq * 64, dtype=BF, device=DEV)).cpu().double().view(want.shape)
+        sees = torch.arange(new[0]) + first >= at
+        assert (y[sees][:, :, 7] == math.inf).all() and (y[sees][:, :, 9] == -math.inf).all(), at
+        near = bound(want, spread, size, n, 64, WEIGHT)
+        off = (y - want).abs() / near
+        others = [d for d in range(64) if d not in (7, 9)]
+        assert off[:, :, others].max() <= 1 and (not (~sees).any() or off[~sees].max() <= 1), at
