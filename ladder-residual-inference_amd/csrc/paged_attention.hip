@@ -439,6 +439,12 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             sc[h][e] = (h ? p1 : p0) >= 0 && 16 * h + 4 * l4 + e < there ? sc[h][e] : -INFINITY;
+        if constexpr (E4M3)   // (a slot that nobody has written holds any byte: 255 is infinity, and their weights are 0)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int n = there - 16 * h - 4 * l4;   // of this lane's four keys, those that there are
+            vs[h] &= n >= 4 ? ~0u : n <= 0 ? 0u : ~0u >> (32 - 8 * n);
+          }
       }
       float top = sc[0][0];
 #pragma unroll

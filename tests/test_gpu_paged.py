@@ -717,3 +717,17 @@ def test_infinite_values_go_through_prompts(hip, lengths, new, hq, hkv):
         off = (y - want).abs() / near
         others = [d for d in range(64) if d not in (7, 9)]
         assert off[:, :, others].max() <= 1 and (not (~sees).any() or off[~sees].max() <= 1), at
+
+
+# ------------------------------------------------------------------------------------------------ what nobody has written
+
+@pytest.mark.parametrize("new", [None, [3, 1, 0, 16, 20, 33]])
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 1, 128), (6, 2, 64)])
+@pytest.mark.parametrize("page,lengths", [(16, [1, 0, 15, 16, 17, 33]), (64, [128, 31, 32, 0, 257, 63]), (256, [513, 255, 0, 1, 20, 40])])
+@pytest.mark.parametrize("byte", [255, 0])
+def test_scales_of_slots_that_no_sequence_has(hip, new, hq, hkv, hd, page, lengths, byte):
+    """Memory that was there already holds any byte behind a sequence's last token: 255 stands for no power of two."""
+    new = None if new is None else [min(a, b) for a, b in zip(new, lengths)]
+    case = Case(lengths, hkv, hd, page, True, seed=54, new=new)
+    case.scales = torch.where(case.scales == 254, torch.tensor(byte, dtype=torch.uint8), case.scales)
+    attend(case, hq)
