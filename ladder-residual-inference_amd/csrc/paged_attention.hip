@@ -757,17 +757,21 @@ struct PagedPrompt {
 // Which rows a block has.
 struct PromptBlock {
   int b, row0, n, ahead, r0;     // sequence, its first row of the call and their number, its tokens ahead of them; the block's first row of the kv head's
+  int held;                      // keys that the table has room for
 };
 // Blocks of a kv head, last ones first (they see the most keys).  false: there are fewer.
 __device__ __forceinline__ bool prompt_block(const PagedCache& c, const PagedBatch& t, int rows, int G, int index, PromptBlock& at) {
   const int lane = threadIdx.x & 63;
   int start = 0, n = 0, ahead = 0, blocks = 0, upto = 0, total = 0;
+  at.held = t.pages << c.shift;
   auto look = [&](int from) {
     const int i = from + lane;
     start = i < t.B ? t.starts[i] : 0;
     n = i < t.B ? t.starts[i + 1] - start : 0;
     n = start < 0 || start > rows || n < 0 ? 0 : n;
-    ahead = (i < t.B ? paged_length(t, c.shift, i) : 0) - n;
+    const int length = i < t.B ? max(t.lengths[i], 0) : 0;   // (positions are the length's, also where the table has not all of its keys)
+    if (length > at.held && t.err) *t.err = LR_DEV_POS_RANGE;
+    ahead = length - n;
     n = min(n, rows - start);   // (a call may have fewer rows than starts says)
     blocks = (int)(((int64_t)n * G + PROMPT_ROWS - 1) / PROMPT_ROWS);
     upto = paged_sums(blocks);
@@ -795,7 +799,7 @@ __device__ __forceinline__ bool prompt_block(const PagedCache& c, const PagedBat
 // keys that the block's last row sees
 __device__ __forceinline__ int prompt_keys(const PromptBlock& at, int G) {
   const int last = min(at.r0 + PROMPT_ROWS, at.n * G) - 1;
-  return max(0, at.ahead + last / G + 1);
+  return max(0, min(at.ahead + last / G + 1, at.held));
 }
 // and into how many parts they are cut
 __device__ __forceinline__ int prompt_parts(int keys, int n_split) { return max(1, min(n_split, prompt_parts_of(keys))); }
@@ -838,9 +842,10 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
   // this lane's row, the last key that it sees, and the smallest and largest of the wave's
   const int n_rows = at.n * G, r = at.r0 + w4 * 32 + col, token = r / G;
   const bool valid = r < n_rows;
-  const int p = valid ? at.ahead + token : -1;
+  const int p = valid ? min(at.ahead + token, at.held - 1) : -1;
   const int wr0 = at.r0 + w4 * 32;
-  const int pmin = __builtin_amdgcn_readfirstlane(at.ahead + wr0 / G), pmax = __builtin_amdgcn_readfirstlane(wr0 < n_rows ? at.ahead + (min(wr0 + 32, n_rows) - 1) / G : -1);
+  const int pmin = __builtin_amdgcn_readfirstlane(min(at.ahead + wr0 / G, at.held - 1));
+  const int pmax = __builtin_amdgcn_readfirstlane(wr0 < n_rows ? min(at.ahead + (min(wr0 + 32, n_rows) - 1) / G, at.held - 1) : -1);
   const int64_t my_row = at.row0 + (valid ? token : 0);
   const int head = kvh * G + (valid ? r - token * G : 0);
 

@@ -59,8 +59,8 @@ def attention(q, k, v, table, lengths, starts, scale):
     n_pages, hkv, page, _ = k.shape
     y = torch.full((rows, hq, hd), math.nan, dtype=F64)
     spread, size = torch.zeros(rows, hq, hd, dtype=F64), 0.0
-    for b, n in enumerate(lengths):
-        n = min(max(n, 0), table.shape[1] * page)
+    for b, length in enumerate(lengths):
+        n = min(max(length, 0), table.shape[1] * page)     # (a position is the length's, whether or not the table has all of the keys)
         first, end = (b, b + 1) if starts is None else (starts[b], starts[b + 1])
         if end <= first:
             continue
@@ -70,7 +70,7 @@ def attention(q, k, v, table, lengths, starts, scale):
         ks, vs = ((x[safe].transpose(0, 1).reshape(hkv, -1, hd)[:, :n] if n else x.new_zeros(hkv, 0, hd)) for x in (k, v))
         vs = torch.where(ok[None, :, None], vs, torch.zeros_like(vs))
         for r in range(first, end):
-            see = ok & (torch.arange(n) <= n - (end - r))
+            see = ok & (torch.arange(n) <= length - (end - r))
             for h in range(hq):
                 kh, vh = ks[h // (hq // hkv)][see], vs[h // (hq // hkv)][see]
                 if not see.any():

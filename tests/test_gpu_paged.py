@@ -731,3 +731,21 @@ def test_scales_of_slots_that_no_sequence_has(hip, new, hq, hkv, hd, page, lengt
     case = Case(lengths, hkv, hd, page, True, seed=54, new=new)
     case.scales = torch.where(case.scales == 254, torch.tensor(byte, dtype=torch.uint8), case.scales)
     attend(case, hq)
+
+
+# ------------------------------------------------------------------------------------------------ lengths and starts that a table or a call does not hold
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("hq,hkv,hd,page,pages,lengths,new", [
+    (4, 2, 64, 16, 4, [70, 64], [10, 5]),               # four rows of sequence 0 have a place
+    (4, 1, 128, 16, 4, [64, 100], [64, 40]), (2, 1, 64, 64, 20, [1300, 1281], [30, 2]), (4, 1, 128, 16, 3, [200], [20]),
+])
+def test_rows_of_a_sequence_longer_than_its_table(hip, e4m3, hq, hkv, hd, page, pages, lengths, new):
+    """A row's position is what the length says, whether or not the table has all of the sequence: the keys that it has are those up to there."""
+    held = [min(n, pages * page) for n in lengths]
+    case = Case(held, hkv, hd, page, e4m3, seed=57, new=new)
+    case.table = case.table[:, :pages].contiguous()
+    case.lengths = lengths
+    attend(case, hq)
+    with pytest.raises(hip.LadderHipError, match="position"):
+        hip.raise_on_device_error(DEV)
