@@ -81,3 +81,32 @@ def attention(q, k, v, table, lengths, starts, scale):
                 y[r, h], spread[r, h] = w @ vh, w @ vh.abs()
                 size = max(size, float((kh.abs() @ q[r, h].to(F64).abs()).max()) * scale)
     return y, spread, size
+
+
+def attention_of_sequences(q, k, v, table, lengths, starts, scale):
+    """attention() of a call with starts, all rows of a sequence and head at once."""
+    rows, hq, hd = q.shape
+    n_pages, hkv, page, _ = k.shape
+    y = torch.full((rows, hq, hd), math.nan, dtype=F64)
+    spread, size = torch.zeros(rows, hq, hd, dtype=F64), 0.0
+    for b, length in enumerate(lengths):
+        first, end = starts[b], starts[b + 1]
+        if end <= first:
+            continue
+        there = min(max(length, 0), table.shape[1] * page)
+        ids = table[b, :-(-there // page)].long()
+        ok = ((ids >= 0) & (ids < n_pages)).repeat_interleave(page)[:there]
+        safe = torch.where((ids >= 0) & (ids < n_pages), ids, torch.zeros_like(ids))
+        see = ok & (torch.arange(there) <= length - end + torch.arange(first, end)[:, None])
+        for h in range(hq):
+            kh, vh = (x[safe, h // (hq // hkv)].reshape(-1, hd)[:there] for x in (k, v))
+            qh = q[first:end, h].to(F64)
+            score = torch.where(see, qh @ kh.t() * scale, -math.inf)
+            top = score.amax(-1, keepdim=True) if there else score.new_zeros(end - first, 1)
+            w = torch.where(see, torch.exp(score - torch.where(top > -math.inf, top, 0.0)), 0.0)
+            total = w.sum(-1, keepdim=True)
+            w = w / torch.where(total > 0, total, 1.0)
+            y[first:end, h], spread[first:end, h] = w @ vh, w @ vh.abs()
+            if there:
+                size = max(size, float((qh.abs() @ kh.abs().t()).max()) * scale)
+    return y, spread, size

@@ -749,3 +749,36 @@ def test_rows_of_a_sequence_longer_than_its_table(hip, e4m3, hq, hkv, hd, page, 
     attend(case, hq)
     with pytest.raises(hip.LadderHipError, match="position"):
         hip.raise_on_device_error(DEV)
+
+
+# ------------------------------------------------------------------------------------------------ long prompts
+
+def long_prompts(hip, lengths, new, hq, hkv, hd, page, e4m3, gone=()):
+    """attend() with the oracle over whole sequences at once; `gone`: (sequence, place in its table) of pages that are not there."""
+    case = Case(lengths, hkv, hd, page, e4m3, seed=55, new=new)
+    for b, i in gone:
+        case.table[b, i] = case.n_pages + 7
+    cache, batch = case.on(DEV, hq)
+    q = rnd(case.rows, hq * hd, seed=56)
+    y = cache.attend(batch, q.to(DEV), torch.empty(case.rows, hq * hd, dtype=BF, device=DEV)).cpu().double().view(-1, hq, hd)
+    if gone:
+        with pytest.raises(hip.LadderHipError, match="page"):
+            hip.raise_on_device_error(DEV)
+    clean = lambda x: torch.nan_to_num(x, nan=0.0)
+    want, spread, size = O.attention_of_sequences(q.view(-1, hq, hd), clean(O.values(case.k, case.scales, 0)), clean(O.values(case.v, case.scales, 1)),
+                                                  case.table, case.lengths, case.starts, hd ** -0.5)
+    off = (y - want).abs() / bound(want, spread, size, max(lengths), hd, WEIGHT)
+    assert off.max() <= 1, f"{off.max():.2f} of what rounding explains"
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lengths,new,hq,hkv,hd,page", [
+    ([1300, 20], [1300, 20], 32, 8, 128, 32), ([2048], [600], 64, 8, 64, 64),                           # four waves: more blocks than CUs
+    ([1100, 0, 700, 1], [90, 0, 400, 1], 32, 16, 64, 64),                                               # eight: a block for more than every other CU, not cut
+    ([1300, 20], [1300, 20], 16, 8, 64, 16), ([2100], [1200], 16, 8, 128, 128),
+])
+def test_long_prompts_that_are_not_cut(hip, e4m3, lengths, new, hq, hkv, hd, page):
+    """Keys beyond the 1024 whose pages a wave holds at a time, in one part; the second time with pages missing on either side of there."""
+    long_prompts(hip, lengths, new, hq, hkv, hd, page, e4m3)
+    if lengths[0] > 1100:
+        long_prompts(hip, lengths, new, hq, hkv, hd, page, e4m3, gone=[(0, 1), (0, 1024 // page), (0, (lengths[0] - 40) // page)])

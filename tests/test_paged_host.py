@@ -177,3 +177,19 @@ def test_more_workgroups_than_a_launch_has_threads_for(hip):
     size = lambda rows, Hq, **c: (lambda d: lib.lr_paged_attention_scratch_bytes(ctypes.byref(d[0]), ctypes.byref(d[1]), rows, Hq))(descs(hip, **c))
     assert size(1 << 20, 1 << 10, n_kv_head=1, B=16) > 0
     assert size(1 << 16, 1 << 10, n_kv_head=1 << 10, B=65535) == 0
+
+
+def test_the_oracles_two_forms_agree():
+    from paged_cases import Case
+
+    for lengths, new, gone in (([40, 33, 0, 5], [20, 33, 0, 1], (0, 1)), ([64, 70], [10, 3], (1, 0)), ([2, 9], [5, 9], (1, 0))):
+        case = Case(lengths, 2, 64, 16, True, new=new)
+        case.table[gone] = case.n_pages
+        if lengths[1] == 70:
+            case.table = case.table[:, :4]
+        q = torch.randn(case.rows, 4 * 64, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+        clean = [torch.nan_to_num(O.values(x, case.scales, i), nan=0.0) for i, x in enumerate((case.k, case.v))]
+        y, spread, size = case.oracle(q, 4)
+        y2, spread2, size2 = O.attention_of_sequences(q.view(-1, 4, 64), *clean, case.table, lengths, case.starts, 64 ** -0.5)
+        assert (y - y2).abs().max() < 1e-12 and (spread - spread2).abs().max() < 1e-12
+        assert size <= size2 + 1e-9      # (it looks at keys that a row does not see, too)
