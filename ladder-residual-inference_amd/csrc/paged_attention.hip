@@ -1329,7 +1329,10 @@ static int launch_prompt(const PagedCache& c, const PagedBatch& t, const PagedQu
   return lr_launch_status();
 }
 
+// (0: refused)
 static size_t paged_scratch(const PagedCache& c, const PagedBatch& t, int hd, bool e4m3, int rows, int Hq) {
+  // (rows times heads and 128 more are 32-bit numbers)
+  if (rows <= 0 || Hq <= 0 || Hq > 65535 || Hq % c.Hkv || (int64_t)rows * Hq > 1 << 30 || (t.starts == nullptr && rows != t.B)) return 0;
   if (t.starts) {
     const PromptPlan p = prompt_plan(c, t, hd, rows, Hq);
     return p.items * p.n_split * p.waves > 0xffffffff / 64 ? 0 : 256 + p.bytes;   // (a grid has fewer than 2^32 threads)
@@ -1343,7 +1346,7 @@ static size_t paged_scratch(const PagedCache& c, const PagedBatch& t, int hd, bo
 extern "C" size_t lr_paged_attention_scratch_bytes(const lr_paged_cache_t* cache, const lr_paged_batch_t* batch, int rows, int Hq) {
   PagedCache c;
   PagedBatch t;
-  if (paged_arguments(cache, batch, c, t) || rows <= 0 || Hq <= 0 || Hq % c.Hkv) return 0;
+  if (paged_arguments(cache, batch, c, t)) return 0;
   return paged_scratch(c, t, cache->head_dim, cache->format == LR_CACHE_E4M3, rows, Hq);
 }
 
@@ -1358,9 +1361,8 @@ extern "C" int lr_paged_attention(const lr_paged_attention_t* desc, lr_stream_t 
   LR_REQUIRE_PTR(scratch);
   const int hd = cache->head_dim;
   const bool e4m3 = cache->format == LR_CACHE_E4M3;
-  if (rows <= 0 || Hq <= 0 || Hq % c.Hkv || (t.starts == nullptr && rows != t.B)) return LR_E_SHAPE;
-  if ((int64_t)rows * Hq > 0x3fffffff) return LR_E_UNSUPPORTED;
-  if (Hq > 65535 || ldq < (int64_t)Hq * hd || ldy < (int64_t)Hq * hd) return LR_E_SHAPE;
+  if (rows <= 0 || Hq <= 0 || Hq > 65535 || Hq % c.Hkv || (t.starts == nullptr && rows != t.B)) return LR_E_SHAPE;
+  if (ldq < (int64_t)Hq * hd || ldy < (int64_t)Hq * hd) return LR_E_SHAPE;
   // (the matrix cores give 0 for sums of some 2^-120: a scale that would lift those to numbers that matter is not served)
   if (!(scale > 0.0f && scale <= 0x1p64f)) return LR_E_SHAPE;
   if (ldq % 8 || ldy % 8) return LR_E_ALIGN;

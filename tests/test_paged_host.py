@@ -193,3 +193,23 @@ def test_the_oracles_two_forms_agree():
         y2, spread2, size2 = O.attention_of_sequences(q.view(-1, 4, 64), *clean, case.table, lengths, case.starts, 64 ** -0.5)
         assert (y - y2).abs().max() < 1e-12 and (spread - spread2).abs().max() < 1e-12
         assert size <= size2 + 1e-9      # (it looks at keys that a row does not see, too)
+
+
+def test_sizes_have_no_scratch_where_the_call_refuses_them(hip):
+    """lr_paged_attention_scratch_bytes and lr_paged_attention agree on every size (its calls have no scratch: none of them is made)."""
+    served = refused = 0
+    for starts in (192, None):
+        for B in (1, 3, 65535):
+            for rows in (-1, 0, 1, 3, 65535, 1 << 20, (1 << 20) + 1, (1 << 31) - 1):
+                for Hq in (-2, 0, 2, 7, 8, 1024, 65534, 65536, 1 << 24):
+                    cache, batch = descs(hip, starts=starts, B=B)
+                    size = hip.load().lr_paged_attention_scratch_bytes(ctypes.byref(cache), ctypes.byref(batch), rows, Hq)
+                    ld = max(Hq, 1) * 128
+                    code = attend(hip, cache, batch, 1 << 20, ld, 1 << 60, ld, rows, Hq, 0.1, 1 << 22, 0)     # (q ends below 2^56)
+                    bad = rows <= 0 or Hq <= 0 or Hq > 65535 or Hq % 2 or (starts is None and rows != B)
+                    big = rows * Hq > 1 << 30
+                    assert (size == 0) == (bad or big), (starts, B, rows, Hq, size)
+                    assert code == (E_SHAPE if bad or not big else E_UNSUPPORTED), (starts, B, rows, Hq, code)    # (not big: no room)
+                    served += size > 0
+                    refused += big and not bad
+    assert served > 20 and refused > 5
