@@ -133,11 +133,16 @@ class PagedKVCache(nn.Module):
         return self._desc
 
     def _apply(self, fn, recurse=True):
-        """Moving the module moves the pages (.to(device), .cuda()); their types stay what they are."""
-        kept = fn
-        fn = lambda t: kept(t).to(t.dtype) if t.dtype in (torch.bfloat16, torch.float8_e4m3fn) else kept(t)
+        """Moving the module moves the pages (.to(device), .cuda()); a cast (.half(), .to(dtype)) leaves their bytes as they are."""
+        def move(t):
+            raw = t.contiguous().view(torch.uint8)
+            to = fn(raw)
+            if to.dtype != torch.uint8:      # (.type() casts whole numbers, too)
+                to = raw.to(to.device)
+            return t if to.device == t.device and to.data_ptr() == t.data_ptr() else to.contiguous().view(t.dtype)
+
         self._desc = None
-        return super()._apply(fn, recurse)
+        return super()._apply(move, recurse)
 
     def batch(self, table: Tensor, lengths: Tensor, n_head: int, starts: Optional[Tensor] = None, rows: Optional[int] = None) -> PagedBatch:
         """table [B, pages], lengths [B] (the call's own tokens among them), starts [B + 1] int32 on the device (None: one row per

@@ -213,3 +213,24 @@ def test_sizes_have_no_scratch_where_the_call_refuses_them(hip):
                     served += size > 0
                     refused += big and not bad
     assert served > 20 and refused > 5
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_casts_leave_the_pages_bytes(dtype):
+    """A model's .half() is not its cache's: every 16-bit (8-bit) number stays what it was, in the same memory."""
+    from gpt_fast.utils import PagedKVCache
+
+    n = 16 * 64
+    raw = torch.arange(64 * n).to(torch.int16).view(torch.uint8) if dtype == torch.bfloat16 else torch.arange(2 * n).to(torch.uint8)
+    pages = lambda: raw.clone().view(dtype).view(-1, 1, 16, 64)
+    scales = None if dtype == torch.bfloat16 else torch.arange(2 * 32).to(torch.uint8).view(2, 1, 2, 16)
+    held = lambda c: [b.contiguous().view(torch.uint8).flatten().tolist() for b in c.buffers()]
+    cache = PagedKVCache.from_pages(pages(), pages(), scales)
+    want, at = held(cache), cache.k_pages.data_ptr()
+    for cast in (lambda m: m.half(), lambda m: m.to(torch.float16), lambda m: m.double(), lambda m: m.to(torch.float32), lambda m: m.bfloat16(),
+                 lambda m: m.type(torch.float16), lambda m: m.to("cpu", torch.half), lambda m: m.cpu()):
+        outer = torch.nn.ModuleDict(dict(cache=cache, other=torch.nn.Linear(2, 2)))
+        cast(outer)
+        assert held(cache) == want and cache.k_pages.dtype == dtype and cache.k_pages.data_ptr() == at
+    cache.to("meta")
+    assert cache.k_pages.device.type == "meta" and cache.k_pages.dtype == dtype and cache.k_pages.shape[1:] == (1, 16, 64)
