@@ -804,6 +804,7 @@ int lr_linear_multi_route(const lr_projection_t* projections, int n_projections,
  * starts[B] on are left as they were, and a call of fewer rows does those.  NULL: one row per sequence (rows == B), its last token; a sequence of length 0 is an empty place.
  * All int32, read on the device (a captured call may be replayed after they have changed there).  Entries of the table behind a
  * sequence's length are not read.  Several sequences may share a page that none of them writes.
+ * A call whose launch would have 2^32 threads or more is LR_E_UNSUPPORTED (2^24 rows at least).
  * Conditions only the device can see set *err (may be NULL): a position outside the table's pages or the angles LR_DEV_POS_RANGE, a page
  * number outside the cache LR_DEV_PAGE_RANGE. */
 enum { LR_CACHE_BF16 = 0, LR_CACHE_E4M3 = 1 };

@@ -251,6 +251,12 @@ static inline int paged_tokens(int rows, int heads, int hd) {
   return n < 1 || most < 1 ? 1 : n > most ? most : n;
 }
 
+// (0: a grid of 2^32 threads or more, which a launch has not)
+static inline unsigned paged_workgroups(int rows, int tokens) {
+  const int64_t n = ((int64_t)rows + tokens - 1) / tokens;
+  return n > 0xffffffff / 256 ? 0 : (unsigned)n;
+}
+
 template <int HD, bool E4M3, bool PAIRS>
 static void launch_write(bool f32, unsigned grid, const PagedCache& c, const PagedBatch& t, const PagedWrite& w, hipStream_t s) {
   if (f32) k_paged_write<HD, E4M3, PAIRS, float><<<dim3(grid), dim3(256), 0, s>>>(c, t, w);
@@ -270,13 +276,14 @@ extern "C" int lr_paged_write(const lr_paged_write_t* desc, lr_stream_t stream) 
   if (rows <= 0 || Hq <= 0 || Hq % c.Hkv || (t.starts == nullptr && rows != t.B)) return LR_E_SHAPE;
   if (Hq > 65535 / 3 || ldqkv < (int64_t)(Hq + 2 * c.Hkv) * hd || ldq < (int64_t)Hq * hd) return LR_E_SHAPE;
   if (ldqkv % 8 || ldq % 8) return LR_E_ALIGN;
+  const int tokens = paged_tokens<PAGED_AHEAD>(rows, Hq + 2 * c.Hkv, hd);
+  const unsigned grid = paged_workgroups(rows, tokens);
+  if (grid == 0) return LR_E_UNSUPPORTED;
   const bool in_place = q == qkv && (ldq == ldqkv || rows == 1);
   if (!in_place && paged_overlap(qkv, ldqkv, q, ldq, rows, (int64_t)(Hq + 2 * c.Hkv) * hd, (int64_t)Hq * hd)) return LR_E_SHAPE;
   if (rope && (rope_len <= 0 || rot <= 0 || rot > hd)) return LR_E_SHAPE;
   if (rope && (rot % 16 || (rope_dtype != LR_BF16 && rope_dtype != LR_F32))) return LR_E_UNSUPPORTED;
-  const int tokens = paged_tokens<PAGED_AHEAD>(rows, Hq + 2 * c.Hkv, hd);
   const PagedWrite w = {(const u16*)qkv, ldqkv, (u16*)q, ldq, rope, rope_len, rot, rows, Hq, tokens};
-  const unsigned grid = (unsigned)((rows + tokens - 1) / tokens);
   const bool f32 = rope_dtype == LR_F32;
   hipStream_t s = (hipStream_t)stream;
   const bool e4m3 = cache->format == LR_CACHE_E4M3;
@@ -300,15 +307,16 @@ extern "C" int lr_paged_read(const lr_paged_read_t* desc, lr_stream_t stream) {
   if (rows <= 0 || (t.starts == nullptr && rows != t.B) || c.Hkv > 65535) return LR_E_SHAPE;
   if (ldk < (int64_t)c.Hkv * hd || ldv < (int64_t)c.Hkv * hd) return LR_E_SHAPE;
   if (ldk % 8 || ldv % 8) return LR_E_ALIGN;
-  if (paged_overlap(k, ldk, v, ldv, rows, (int64_t)c.Hkv * hd, (int64_t)c.Hkv * hd)) return LR_E_SHAPE;
   const int tokens = paged_tokens<PAGED_AHEAD_READ>(rows, 2 * c.Hkv, hd);
+  const unsigned grid = paged_workgroups(rows, tokens);
+  if (grid == 0) return LR_E_UNSUPPORTED;
+  if (paged_overlap(k, ldk, v, ldv, rows, (int64_t)c.Hkv * hd, (int64_t)c.Hkv * hd)) return LR_E_SHAPE;
   const PagedRead r = {(u16*)k, (u16*)v, ldk, ldv, rows, tokens};
-  const dim3 grid((unsigned)((rows + tokens - 1) / tokens));
   hipStream_t s = (hipStream_t)stream;
   const bool e4m3 = cache->format == LR_CACHE_E4M3;
-  if (hd == 128 && e4m3) k_paged_read<128, true><<<grid, dim3(256), 0, s>>>(c, t, r);
-  else if (hd == 128) k_paged_read<128, false><<<grid, dim3(256), 0, s>>>(c, t, r);
-  else if (e4m3) k_paged_read<64, true><<<grid, dim3(256), 0, s>>>(c, t, r);
-  else k_paged_read<64, false><<<grid, dim3(256), 0, s>>>(c, t, r);
+  if (hd == 128 && e4m3) k_paged_read<128, true><<<dim3(grid), dim3(256), 0, s>>>(c, t, r);
+  else if (hd == 128) k_paged_read<128, false><<<dim3(grid), dim3(256), 0, s>>>(c, t, r);
+  else if (e4m3) k_paged_read<64, true><<<dim3(grid), dim3(256), 0, s>>>(c, t, r);
+  else k_paged_read<64, false><<<dim3(grid), dim3(256), 0, s>>>(c, t, r);
   return lr_launch_status();
 }

@@ -234,3 +234,12 @@ def test_casts_leave_the_pages_bytes(dtype):
         assert held(cache) == want and cache.k_pages.dtype == dtype and cache.k_pages.data_ptr() == at
     cache.to("meta")
     assert cache.k_pages.device.type == "meta" and cache.k_pages.dtype == dtype and cache.k_pages.shape[1:] == (1, 16, 64)
+
+
+def test_more_rows_than_a_launch_has_threads_for(hip):
+    """2^24 workgroups of 256: a write of many heads and a read of 16 kv heads have one token each."""
+    cache, batch = descs(hip, n_kv_head=16)
+    ld = 64 * 128
+    for rows in (1 << 24, (1 << 31) - 1):
+        assert write(hip, cache, batch, 1 << 20, ld, 1 << 60, ld, rows, 32, None, 0, 0, 1, 0) == E_UNSUPPORTED
+        assert read(hip, cache, batch, 1 << 20, ld, 1 << 60, ld, rows) == E_UNSUPPORTED
