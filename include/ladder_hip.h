@@ -799,9 +799,9 @@ int lr_linear_multi_route(const lr_projection_t* projections, int n_projections,
  * read back is exact in bf16.  page: a power of two from 16 to 256; head_dim 64 or 128; n_pages * n_kv_head below 2^31 (LR_E_UNSUPPORTED otherwise).
  *
  * A batch is B sequences: table [B, pages] (row stride ld_table) names their pages in order, lengths [B] how many tokens they have,
- * the call's own among them.  starts [B + 1], ascending from 0: the call's rows starts[b] .. starts[b + 1] - 1 are the last tokens of
- * sequence b, in order, i.e. row r is at position lengths[b] - starts[b + 1] + r; none for a sequence that takes no part; rows from
- * starts[B] on are left as they were, and a call of fewer rows does those.  NULL: one row per sequence (rows == B), its last token; a sequence of length 0 is an empty place.
+ * the call's own among them.  starts [B + 1], ascending, from 0 on: the call's rows starts[b] .. starts[b + 1] - 1 are the last tokens of
+ * sequence b, in order, i.e. row r is at position lengths[b] - starts[b + 1] + r; none for a sequence that takes no part; rows ahead of starts[0] and
+ * from starts[B] on are left as they were, and a call of fewer rows does those.  NULL: one row per sequence (rows == B), its last token; a sequence of length 0 is an empty place.
  * All int32, read on the device (a captured call may be replayed after they have changed there).  Entries of the table behind a
  * sequence's length are not read.  Several sequences may share a page that none of them writes.
  * A call whose launch would have 2^32 threads or more is LR_E_UNSUPPORTED (2^24 rows at least).

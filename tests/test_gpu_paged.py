@@ -782,3 +782,26 @@ def test_long_prompts_that_are_not_cut(hip, e4m3, lengths, new, hq, hkv, hd, pag
     long_prompts(hip, lengths, new, hq, hkv, hd, page, e4m3)
     if lengths[0] > 1100:
         long_prompts(hip, lengths, new, hq, hkv, hd, page, e4m3, gone=[(0, 1), (0, 1024 // page), (0, (lengths[0] - 40) // page)])
+
+
+def test_rows_ahead_of_the_first_sequence_are_left_alone(hip):
+    """starts[0] beyond 0: by write, read and attention alike."""
+    hq, hkv, hd, page = 4, 1, 64, 16
+    case = Case([40, 33], hkv, hd, page, False, seed=58, new=[4, 33])
+    cache, batch = case.on(DEV, hq, rows=case.rows + 3)
+    batch.starts.add_(3)
+    n = case.rows + 3
+    qkv = rnd(n, (hq + 2 * hkv) * hd, seed=59).to(DEV)
+    q = torch.full((n, hq * hd), 3.0, dtype=BF, device=DEV)
+    k0 = cache.k_pages.clone()
+    cache.write(batch, qkv, q)
+    assert (q[:3] == 3).all() and torch.equal(q[3:], qkv[3:, :hq * hd])
+    for r, _, pos, p, s in O.places(case.table, case.lengths, [3, 7, 40], page):
+        k0[p, :, s] = qkv[r, hq * hd:(hq + hkv) * hd].view(hkv, hd)
+    assert torch.equal(bits(cache.k_pages), bits(k0))
+    k, v = (torch.full((n, hkv * hd), 5.0, dtype=BF, device=DEV) for _ in range(2))
+    cache.read(batch, k, v)
+    assert (k[:3] == 5).all() and (v[:3] == 5).all() and torch.equal(k[3:], qkv[3:, hq * hd:(hq + hkv) * hd])
+    y = torch.full_like(q, 7)
+    cache.attend(batch, q, y)
+    assert (y[:3] == 7).all() and y[3:].isfinite().all()
