@@ -58,6 +58,9 @@ class KVCache(nn.Module):
         return self.k_cache, self.v_cache
 
 
+_PAGED_SHAPES = {}
+
+
 class PagedBatch:
     """Sequences of one call on paged caches of one shape (PagedKVCache.batch): table, lengths and starts on the device, and the
     scratch of the attention.  The tensors may be written between calls, also between replays of a captured graph, and are not replaced;
@@ -66,7 +69,7 @@ class PagedBatch:
 
     def __init__(self, cache: "PagedKVCache", table: Tensor, lengths: Tensor, n_head: int, starts: Optional[Tensor], rows: int):
         self.table, self.lengths, self.starts, self.n_head, self.rows = table, lengths, starts, n_head, rows
-        self.shape = cache.shape
+        self.shape = cache.desc() and cache._shape
         assert table.device == cache.k_pages.device, "the tables are where the pages are"
         if table.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a batch is made ahead of a graph's capture: its scratch is cleared once, and kept")
@@ -129,7 +132,8 @@ class PagedKVCache(nn.Module):
     def desc(self):
         if self._desc is None:
             self._desc = _hip.paged_cache_desc(self.k_pages, self.v_pages, self.scales)
-            self._shape = self.shape
+            self._shape = _PAGED_SHAPES.setdefault(self.shape, self.shape)     # (one tuple each: a call's check compares addresses)
+            self._at = self.k_pages.data_ptr(), self.v_pages.data_ptr(), None if self.scales is None else self.scales.data_ptr()
         return self._desc
 
     def _apply(self, fn, recurse=True):
@@ -149,11 +153,18 @@ class PagedKVCache(nn.Module):
         sequence); `rows`: how many rows a call has at most (given with starts).  Serves every cache of the same shape."""
         assert starts is None or rows is not None, "with starts, say how many rows a call has at most"
         assert starts is not None or rows in (None, table.shape[0]), "without starts there is one row per sequence"
+        self._desc = None     # (the pages as they are now)
         return PagedBatch(self, table, lengths, n_head, starts, table.shape[0] if rows is None else rows)
 
     def _check(self, batch: PagedBatch):
-        desc = self._desc or self.desc()
-        if batch.shape != self._shape:
+        desc = self._desc
+        if desc is not None:     # (pages may be exchanged behind __setattr__, too: .data, set_(), a shallow copy's buffers)
+            b, (k, v, s) = self._buffers, self._at
+            if b["k_pages"].data_ptr() != k or b["v_pages"].data_ptr() != v or s is not None and b["scales"].data_ptr() != s:
+                desc = self._desc = None
+        if desc is None:
+            desc = self.desc()
+        if batch.shape is not self._shape:
             raise ValueError(f"a batch for pages {batch.shape}: got pages {self._shape}")
         return desc
 

@@ -805,3 +805,43 @@ def test_rows_ahead_of_the_first_sequence_are_left_alone(hip):
     y = torch.full_like(q, 7)
     cache.attend(batch, q, y)
     assert (y[:3] == 7).all() and y[3:].isfinite().all()
+
+
+def test_pages_exchanged_under_a_cache(hip):
+    """Whichever way another tensor comes into the cache's place, calls go to that one."""
+    import copy
+    hq = 4
+    cases = [Case([40, 33], 2, 64, 16, e4m3, seed=s) for e4m3 in (False, True) for s in (61, 62)]
+    for first, second in (cases[:2], cases[2:]):
+        cache, batch = first.on(DEV, hq)
+        batch.table.copy_(second.table)
+        other, _ = second.on(DEV, hq)
+        q = rnd(2, hq * 64).to(DEV)
+        attended = lambda c: c.attend(batch, q, torch.empty_like(q))
+        want, kept = attended(other), [b for b in cache.buffers()]
+        assert not torch.equal(attended(cache), want)
+        names = ["k_pages", "v_pages"] + ([] if cache.scales is None else ["scales"])
+
+        def restore():
+            for n, t in zip(names, kept):
+                setattr(cache, n, t)
+            assert not torch.equal(attended(cache), want)
+
+        for n in names:
+            setattr(cache, n, getattr(other, n))
+        assert torch.equal(attended(cache), want)
+        restore()
+        for n in names:
+            cache._buffers[n] = getattr(other, n)
+        assert torch.equal(attended(cache), want)
+        restore()
+        twin = copy.copy(cache)
+        for n in names:
+            setattr(twin, n, getattr(other, n))
+        assert torch.equal(attended(twin), attended(cache))      # (a shallow copy has the same buffers)
+        restore()
+        old = [t.data for t in kept]                            # (the memory stays while the tensors have other)
+        for n in names:
+            getattr(cache, n).data = getattr(other, n)
+        assert torch.equal(attended(cache), want)
+        del old
