@@ -65,7 +65,8 @@ class PagedBatch:
     """Sequences of one call on paged caches of one shape (PagedKVCache.batch): table, lengths and starts on the device, and the
     scratch of the attention.  The tensors may be written between calls, also between replays of a captured graph, and are not replaced;
     calls that may overlap have batches of their own.  Like any tensor it is made on the current stream, ahead of a capture: work on
-    another stream waits for that one first."""
+    another stream waits for that one first.  It is kept as long as a graph that has captured a call with it; given up otherwise, its memory is
+    used again when the calls on whatever stream have ended."""
 
     def __init__(self, cache: "PagedKVCache", table: Tensor, lengths: Tensor, n_head: int, starts: Optional[Tensor], rows: int):
         self.table, self.lengths, self.starts, self.n_head, self.rows = table, lengths, starts, n_head, rows
@@ -79,6 +80,7 @@ class PagedBatch:
             raise _hip.LadderHipError(f"a paged cache of pages {cache.shape} is not served with {n_head} q heads and a table "
                                       f"{tuple(table.shape)}: head_dim 64 or 128, pages of 16 to 256 tokens (a power of two)")
         scratch = torch.zeros(need, dtype=torch.uint8, device=table.device)
+        self.desc.tensors.append(scratch)
         self.room = scratch.data_ptr(), need
         self.scratch = scratch
 

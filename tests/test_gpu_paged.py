@@ -845,3 +845,36 @@ def test_pages_exchanged_under_a_cache(hip):
             getattr(cache, n).data = getattr(other, n)
         assert torch.equal(attended(cache), want)
         del old
+
+
+def test_a_batch_given_up_while_another_stream_works(hip):
+    """Its memory and that of its tables is not handed out before the work has ended: later tensors of the same sizes lie elsewhere."""
+    case = Case([3000, 900], 2, 128, 16, False, seed=63)
+    q = rnd(2, 8 * 128).to(DEV)
+    cache, first = case.on(DEV, 8)
+    want = cache.attend(first, q, torch.empty_like(q)).clone()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        y = torch.empty_like(q)
+        i = lambda x: torch.as_tensor(x, dtype=torch.int32).to(DEV)
+        batch = cache.batch(i(case.table), i(case.lengths), 8)
+        tensors = [batch.table, batch.lengths, batch.scratch]
+        sizes, at = [(t.shape, t.dtype) for t in tensors], {t.data_ptr() for t in tensors}
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            cache.attend(batch, q, y)
+        del batch, tensors
+        later = [torch.full(shape, 77, dtype=dtype, device=DEV) for shape, dtype in sizes for _ in range(4)]
+        assert not side.query() and not at & {t.data_ptr() for t in later}
+        side.synchronize()
+        assert torch.equal(y, want)
+        del later
+    # in a graph: captured with a batch made before, replayed while that is kept
+    graph, y = torch.cuda.CUDAGraph(), torch.empty_like(q)
+    with torch.cuda.graph(graph):
+        cache.attend(first, q, y)
+    for _ in range(3):
+        y.zero_()
+        graph.replay()
+        assert torch.equal(y, want)
