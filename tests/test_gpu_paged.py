@@ -8,6 +8,7 @@ import torch
 
 from oracle import paged_oracle as O
 from paged_cases import BF, E4M3, F32, F64, Case, bound
+from paged_schedule import SCHEDULED
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -878,3 +879,14 @@ def test_a_batch_given_up_while_another_stream_works(hip):
         y.zero_()
         graph.replay()
         assert torch.equal(y, want)
+
+
+# ------------------------------------------------------------------------------------------------ how a step is dealt out
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lengths,hq,hkv,hd,page,way", SCHEDULED, ids=[f"{c[5]}{i}" for i, c in enumerate(SCHEDULED)])
+def test_every_way_of_dealing_out_a_step(hip, e4m3, lengths, hq, hkv, hd, page, way):
+    """The ways that tests/paged_schedule.py tells apart, each against the oracle; the same bits the second time."""
+    cache, batch, q, got = attend(Case(lengths, hkv, hd, page, e4m3, seed=64), hq)
+    again = cache.attend(batch, q.to(DEV), torch.empty(len(lengths), hq * hd, dtype=BF, device=DEV))
+    assert torch.equal(again.cpu().double().view(got.shape), got)

@@ -243,3 +243,20 @@ def test_more_rows_than_a_launch_has_threads_for(hip):
     for rows in (1 << 24, (1 << 31) - 1):
         assert write(hip, cache, batch, 1 << 20, ld, 1 << 60, ld, rows, 32, None, 0, 0, 1, 0) == E_UNSUPPORTED
         assert read(hip, cache, batch, 1 << 20, ld, 1 << 60, ld, rows) == E_UNSUPPORTED
+
+
+def test_the_batches_of_the_gpu_tests_take_every_way():
+    """What the steps of tests/test_gpu_paged.py over SCHEDULED are there for, worked out from the rules."""
+    from paged_schedule import SCHEDULED, facts, workers_of
+
+    got = []
+    for lengths, hq, hkv, hd, page, way in SCHEDULED:
+        f = facts(lengths, workers_of(len(lengths), max(-(-n // page) for n in lengths) + 1, page, hq, hkv, hd))
+        assert f[0] == way, (f, way)
+        got.append((len(lengths) <= 64, *f))
+    assert any(few and way == "line" and two == 2 for few, way, _, _, two, _ in got)                   # two open parts, up to 64 sequences
+    assert any(not few and way == "line" and two == 2 for few, way, _, _, two, _ in got)               # and beyond
+    assert any(few and way == "line" and n >= w for few, way, n, w, _, _ in got)                       # more sequences than workers, as a line
+    assert sum(way == "whole" and n > w for _, way, n, w, _, _ in got) == 2                            # and whole
+    assert any(way == "cut" and parts > 32 for _, way, _, _, _, parts in got)                          # joined in blocks
+    assert any(way == "line" and parts > 32 for _, way, _, _, _, parts in got)
