@@ -796,7 +796,8 @@ int lr_linear_multi_route(const lr_projection_t* projections, int n_projections,
  * A cache holds k and v, [n_pages, n_kv_head, page, head_dim], in bf16 or e4m3 (float8_e4m3fn).  An e4m3 row is x / 2^e rounded
  * once, e the smallest exponent with max|x| <= 448 * 2^e over the row's finite values (at least -126; what is not finite is NaN);
  * scales [n_pages, n_kv_head, 2, page] holds e + 127 as a byte, those of a page's keys, then those of its values.  What is
- * read back is exact in bf16.  page: a power of two from 16 to 256; head_dim 64 or 128; n_pages * n_kv_head below 2^31 (LR_E_UNSUPPORTED otherwise).
+ * read back is exact in bf16 but at the ends of its range: numbers below 2^-133 are rounded to multiples of that, finite ones from
+ * 248 * 2^120 on were rounded to 2^128, which bf16 has as infinity.  page: a power of two from 16 to 256; head_dim 64 or 128; n_pages * n_kv_head below 2^31 (LR_E_UNSUPPORTED otherwise).
  *
  * A batch is B sequences: table [B, pages] (row stride ld_table) names their pages in order, lengths [B] how many tokens they have,
  * the call's own among them.  starts [B + 1], ascending, from 0 on: the call's rows starts[b] .. starts[b + 1] - 1 are the last tokens of
@@ -856,7 +857,8 @@ int lr_paged_read(const lr_paged_read_t* desc, lr_stream_t stream);
  * Hq / n_kv_head; q, y [rows, Hq head_dim] (row strides ldq, ldy) with no memory in common.  The cache holds the call's tokens already.
  * A row that sees no key is zeros; keys of a page out of range, and those behind the table's pages, count as not there; what keys that a
  * row does not see hold, NaN too, does not reach it.  Scores, softmax and sums in fp32; a weight enters the matrix cores as two bf16
- * numbers (2^-16 of it is lost), as in lr_attn_prefill; one rounding of y.  scale: positive, up to 2^64.
+ * numbers (2^-16 of it is lost), as in lr_attn_prefill; one rounding of y.  scale: positive, up to 2^64.  Weights are
+ * up to 2^8 before they are divided by their sum, so sums may overflow where |v| times the number of keys passes 2^119.
  * scratch: lr_paged_attention_scratch_bytes() (0: sizes that are refused), zero before the first call and kept for calls with the same
  * cache but for its addresses and n_pages, the same B, pages, Hq and starts or none (rows no more than those it was sized for), one
  * after the other: calls that may overlap have their own. */

@@ -890,3 +890,43 @@ def test_every_way_of_dealing_out_a_step(hip, e4m3, lengths, hq, hkv, hd, page, 
     cache, batch, q, got = attend(Case(lengths, hkv, hd, page, e4m3, seed=64), hq)
     again = cache.attend(batch, q.to(DEV), torch.empty(len(lengths), hq * hd, dtype=BF, device=DEV))
     assert torch.equal(again.cpu().double().view(got.shape), got)
+
+
+# ------------------------------------------------------------------------------------------------ bytes
+
+def test_every_byte_with_every_power_is_read_back(hip):
+    """All 256 e4m3 numbers with all powers that a write gives: the values they stand for, which are bf16 numbers but below 2^-133 and from 2^128 on."""
+    from gpt_fast.utils import PagedKVCache
+    hd, page = 128, 256
+    codes = torch.arange(256, dtype=torch.uint8).view(2, 1, 1, hd).expand(2, 1, page, hd).contiguous()      # page 0: codes 0..127, 1: the rest
+    scales = torch.arange(256, dtype=torch.uint8).clamp(1, 247).view(1, 1, 1, page).expand(2, 1, 2, page).contiguous()
+    cache = PagedKVCache.from_pages(codes.view(E4M3).to(DEV), codes.view(E4M3).to(DEV), scales.to(DEV))
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    batch = cache.batch(i(0, 1)[None], i(512), 1, starts=i(0, 512), rows=512)
+    k, v = (torch.empty(512, hd, dtype=BF, device=DEV) for _ in range(2))
+    cache.read(batch, k, v)
+    want = O.values(codes.view(E4M3), scales, 0).reshape(512, hd).to(F32).to(BF)
+    for got in (k.cpu(), v.cpu()):
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(torch.nan_to_num(got, nan=0.0), torch.nan_to_num(want, nan=0.0))
+
+
+def test_rows_of_the_largest_and_smallest_numbers_are_written_as_defined(hip):
+    """At both ends of bf16's range: the exponent and the rounding as the definition says, read back as bf16 rounds what is kept."""
+    hd = 64
+    qkv = torch.zeros(4, 3 * hd, dtype=BF)
+    most = torch.finfo(BF).max
+    qkv[0, hd:] = torch.linspace(-1, 1, 2 * hd).to(BF) * most
+    qkv[1, hd:] = torch.linspace(-1, 1, 2 * hd).to(BF) * 2.0 ** -118
+    qkv[2, hd:] = torch.arange(2 * hd, dtype=torch.int16).view(BF)                # subnormal numbers: multiples of 2^-133
+    qkv[3, hd:] = torch.tensor([248.0, 247.0]).to(BF).repeat(hd) * 2.0 ** 120
+    case = Case([4], 1, hd, 16, True, new=[4])
+    cache, batch = case.on(DEV, 1)
+    cache.write(batch, qkv.to(DEV), torch.empty(4, hd, dtype=BF, device=DEV))
+    k, v = (torch.empty(4, hd, dtype=BF, device=DEV) for _ in range(2))
+    cache.read(batch, k, v)
+    page = int(case.table[0, 0])
+    for which, (pages, got) in enumerate(((cache.k_pages, k), (cache.v_pages, v))):
+        x, byte = O.quantise(qkv[:, (1 + which) * hd:(2 + which) * hd].float())
+        assert torch.equal(cache.scales[page, 0, which, :4].cpu(), byte) and torch.equal(pages[page, 0, :4].cpu().float(), x.float())
+        want = (x.double() * torch.exp2(byte.double() - 127)[:, None]).to(F32).to(BF)
+        assert torch.equal(got.cpu(), want) and want[0].isinf().any() and want[3].isinf().any() and want[1:3].isfinite().all()
