@@ -18,7 +18,7 @@ OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "gpt_fast", "libladder_hip.so")
 PROF_LIB = os.path.join(HERE, "gpt_fast", "libladder_hip_prof.so")
 BAND_PROF_LIB = os.path.join(HERE, "gpt_fast", "libladder_hip_bandprof.so")
-HEADERS = [os.path.join(CSRC, h) for h in ("lr_common.h", "mixer_common.h", "attn_decode_item.h", "paged_common.h", "stream_band.h")] + \
+HEADERS = [os.path.join(CSRC, h) for h in ("lr_common.h", "mixer_common.h", "attention_common.h", "attn_decode_item.h", "paged_common.h", "stream_band.h")] + \
     [os.path.join(HERE, "..", "include", "ladder_hip.h")]
 # sources that compile another source under a switch
 INCLUDES = {"ladder_step_fp8.hip": [os.path.join(CSRC, "ladder_step.hip")]}

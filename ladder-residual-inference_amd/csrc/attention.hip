@@ -14,6 +14,7 @@
 // output in registers, K/V tiles of 32 keys broadcast from LDS as fp32).  Both: exact fp32
 // softmax semantics, one rounding of the output.
 #include "lr_common.h"
+#include "attention_common.h"
 #include "attn_decode_item.h"
 #include <atomic>
 
@@ -247,15 +248,6 @@ __global__ __launch_bounds__(64) void k_attn_prefill(const u16* __restrict__ q, 
 // (p = bf16(p) + bf16(p - bf16(p))), which keeps the fp32 softmax weights to ~2^-17: the result matches
 // the fp32 "math" attention of the eager reference (utils.py:247-258) to rounding of the final bf16.
 // A workgroup is 4 waves = NWH heads of one kv head x NWQ tiles of 32 queries sharing the K / V tiles.
-// e^x through the hardware exp2 (1 ulp in fp32: far below the bf16 rounding of the output), with the score scale
-// folded into its argument; the library expf costs ~15 VALU instructions, and this kernel is VALU-bound next to
-// its MFMAs
-// max(a, b) as the median of {a, b, +inf}: one instruction (fmaxf makes the compiler canonicalise both operands
-// first, an instruction each, when they come out of a matrix-core product).  Not for NaN operands.
-// (No inline assembler here: the compiler does not count the wait states between a matrix-core instruction and
-// an assembler statement that reads its result, and the statement then reads the registers too early.)
-__device__ __forceinline__ float max_med3(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
-__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 constexpr float PREFILL_TAU2 = 8.0f;  // log2 of the largest softmax weight before the reference point moves
 
 struct WindowKeys {
@@ -289,7 +281,6 @@ struct WindowKeys {
 // conflicts.  Before (32 keys in one LDS buffer through registers, V transposed on its way in, two barriers) / now, us: 32 heads of 128,
 // 8 kv heads: 8 x 2048 tokens 460 / 396 (598 / 694 TFLOP/s of products), 4 x 1300 112 / 96, 2 x 1000 50.8 / 35.9, 777 28.4 / 22.4, 300 14.0 / 12.1,
 // 100 8.2 / 8.2, 32 6.3 / 6.4, 16 5.6 / 5.7; of 64: 4 x 1024 59.9 / 40.1, 512 15.1 / 11.8, 100 6.3 / 5.8, 32 4.8 / 4.7.
-typedef int i32x4_t __attribute__((ext_vector_type(4)));
 constexpr int PREFILL_PARTS_FROM = 512, PREFILL_HALF_TO = 128;   // keys that are seen, see above
 enum { PREFILL_WHOLE, PREFILL_HALF, PREFILL_EACH };
 template <int HD, int KSP, int KEYS>
@@ -298,13 +289,6 @@ struct PrefillLds {
   static constexpr int MERGE = KSP == 2 ? 4 * (HD / 2 + 2) * 64 * 4 : 0;
   static constexpr int KMAX = 2 * STAGE > MERGE ? 2 * STAGE : MERGE, BYTES = KMAX + 32;   // (KMAX: an int of each of up to eight waves)
 };
-// the place among a row's pieces is the piece's number XOR this: 16 lanes reading one piece of 16 consecutive keys, and 16 reading four
-// neighbouring pieces (32 dimensions) of four keys, touch every bank once
-template <int HD>
-__device__ __forceinline__ int key_swizzle(int key) { return HD == 128 ? key & 15 : (key >> 1) & 7; }
-template <int HD>
-__device__ __forceinline__ int value_swizzle(int key) { return HD == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2; }
-
 // WIN (lr_window_attention): a sliding window, the score scale as an argument, and the kv heads' keys and values side by
 // side as rows of a matrix, in the order lr_latent_window gives them; head sizes up to HD.
 template <int HD, int NWH, int KSP, int KEYS, int HALF, bool WIN>

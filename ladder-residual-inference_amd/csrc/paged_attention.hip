@@ -1,11 +1,10 @@
 // lr_paged_attention: softmax attention of a call's rows on the pages of a key-value cache.
+#include "attention_common.h"
 #include "paged_common.h"
 
 #include <atomic>
 #include <cfloat>
 #include <type_traits>
-
-typedef short i16x4_t __attribute__((ext_vector_type(4)));
 
 struct PagedQuery {
   const u16* q;
@@ -33,9 +32,7 @@ struct PagedQuery {
 // of these 43.6, 50, 58), rows that nobody else reads come non-temporally (10 %).  Few keys: a chain of waits, 8.4 us at first for one sequence of 2048
 // and one kv head, 7.3 now: the lengths 0.7, page numbers and q 1.1, keys, values and products 1.5, four waves' results 0.9, what a worker leaves
 // and its ticket 1.0, the parts together 1.8, the rest the launch.
-typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x2_t __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 constexpr float PAGED_TAU2 = 8.0f;   // log2 of the largest weight before the reference point of the exponentials moves
 constexpr int PAGED_OUT = (int)0x80000000;   // an offset outside every resource: comes as zeros
 constexpr int PAGED_COHERENT = 17;   // sc0 sc1: past this XCD's L2
@@ -810,13 +807,6 @@ struct PromptLds {
   static constexpr int MERGE = KSP == 2 ? 4 * (HD / 2 + 2) * 64 * 4 : 0;
   static constexpr int BYTES = 2 * STAGE > MERGE ? 2 * STAGE : MERGE;
 };
-// the place among a row's 16-byte pieces is the piece's number XOR this: 16 lanes reading one piece of 16 consecutive keys, and 16 reading
-// four neighbouring pieces of four keys, touch every bank once
-template <int HD>
-__device__ __forceinline__ int prompt_k_place(int key) { return HD == 128 ? key & 15 : (key >> 1) & 7; }
-template <int HD>
-__device__ __forceinline__ int prompt_v_place(int key) { return HD == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2; }
-
 // KSP 2: eight waves, the second four the second 32 keys of every portion for the same rows; their results meet in LDS.
 template <int HD, bool E4M3, int KSP, bool SPLIT>
 __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache c, const PagedBatch t, const PagedPrompt a) {
@@ -898,8 +888,8 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
   const u32 lds0 = __builtin_amdgcn_readfirstlane((u32)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)prompt_lds);
   const int lrow = lane / PIECES, place = lane % PIECES;
   static_assert(NW * RPL % 16 == 0 && RPL % 4 == 0, "a lane's piece is the same for all of a wave's loads");
-  const int kvoff = lrow * RB + (place ^ prompt_k_place<HD>(wave * RPL + lrow)) * 16;
-  const int vvoff = lrow * RB + (place ^ prompt_v_place<HD>(lrow)) * 16;
+  const int kvoff = lrow * RB + (place ^ key_swizzle<HD>(wave * RPL + lrow)) * 16;
+  const int vvoff = lrow * RB + (place ^ value_swizzle<HD>(lrow)) * 16;
   // (with few scalar instructions per load, which a wave issues one by one beside everything else: 150 for the eight of a portion, now 70; 143.5 -> 141 us)
   auto stage_as = [&](auto WHOLE, int t0, int buf) {
     const int group0 = (t0 - groups0 + wave * RPL) >> 4;
@@ -946,7 +936,7 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
                           __builtin_bit_cast(u32, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true)));
       };
       unsigned char* const to = prompt_lds + buf * L::STAGE + value * L::TILE + key * RB;
-      const int swap = value ? prompt_v_place<HD>(key) : prompt_k_place<HD>(key);
+      const int swap = value ? value_swizzle<HD>(key) : key_swizzle<HD>(key);
       *reinterpret_cast<uint4*>(to + ((2 * pc) ^ swap) * 16) = two(raw[i].x, raw[i].y);
       *reinterpret_cast<uint4*>(to + ((2 * pc + 1) ^ swap) * 16) = two(raw[i].z, raw[i].w);
     }
@@ -954,13 +944,13 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
 
   // where this lane reads: the K fragments of key `col` of a tile (k-step i: XOR 32 i), and 4 dimensions of key (lane % 16) / 4 of the
   // four keys whose values 16 lanes exchange (32-row tile d of O^T)
-  const int kat = (part * 32 + col) * RB + ((half ^ prompt_k_place<HD>(col)) * 16);
+  const int kat = (part * 32 + col) * RB + ((half ^ key_swizzle<HD>(col)) * 16);
   const int vkey = (lane & 15) >> 2;
   int vat[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) {
     const int piece = 4 * d + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-    vat[d] = L::TILE + (part * 32 + 4 * half + vkey) * RB + (piece ^ prompt_v_place<HD>(vkey)) * 16 + (lane & 1) * 8;
+    vat[d] = L::TILE + (part * 32 + 4 * half + vkey) * RB + (piece ^ value_swizzle<HD>(vkey)) * 16 + (lane & 1) * 8;
   }
   // this wave's tiles of 32 keys of the portion at t0
   auto tiles = [&](int t0, int buf) {
@@ -998,7 +988,7 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
     }
     float top = sacc[0][0];
 #pragma unroll
-    for (int v = 1; v < 16 * N; ++v) top = __builtin_amdgcn_fmed3f(top, sacc[v / 16][v % 16], INFINITY);   // (the larger of two: one instruction, where fmaxf takes a second that makes NaN quiet)
+    for (int v = 1; v < 16 * N; ++v) top = max_med3(top, sacc[v / 16][v % 16]);   // (a row that sees NaN is NaN, whatever this is)
     {
       const u32 u = __float_as_uint(top);
       const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
