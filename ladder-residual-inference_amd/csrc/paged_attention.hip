@@ -27,11 +27,11 @@ struct PagedQuery {
 // is free, hands them on as the second product's operand without moving them.  Weights enter as two bf16 numbers (2^-16 of the
 // weight).  e4m3: K is expanded with its row's power of two on the way to the product, V without, its power goes into the weight.
 //
-// Bound: memory.  64 sequences of 2048 keys, 8 kv heads of 128, e4m3: 43.4 us, 6.3 TB/s (a plain read 7.0); one of 131072 in bf16 85.5 us, 6.3 TB/s;
-// 24 of 1 to 4096 26.6 us.  One workgroup per CU with four waves whose tiles are all in flight reads faster than two or three smaller ones (the first
+// Bound: memory.  64 sequences of 2048 keys, 8 kv heads of 128, e4m3: 43.4 us, 6.3 TB/s (a plain read 7.0); one of 131072 in bf16 84.0 us, 6.4 TB/s;
+// 24 of 1 to 4096 26.4 us.  One workgroup per CU with four waves whose tiles are all in flight reads faster than two or three smaller ones (the first
 // of these 43.6, 50, 58), rows that nobody else reads come non-temporally (10 %).  Few keys: a chain of waits, 8.4 us at first for one sequence of 2048
 // and one kv head, 7.3 now: the lengths 0.7, page numbers and q 1.1, keys, values and products 1.5, four waves' results 0.9, what a worker leaves
-// and its ticket 1.0, the parts together 1.8, the rest the launch.
+// and its ticket 1.0, the parts together 1.8, the rest start and end.
 typedef int i32x2_t __attribute__((ext_vector_type(2)));
 constexpr float PAGED_TAU2 = 8.0f;   // log2 of the largest weight before the reference point of the exponentials moves
 constexpr int PAGED_OUT = (int)0x80000000;   // an offset outside every resource: comes as zeros
@@ -728,8 +728,9 @@ static int launch_paged_decode(const PagedCache& c, const PagedBatch& t, const P
 // from there on the two are the same.
 // Few rows: a workgroup's keys are cut among several, whose results a second launch puts together.
 //
-// Bound: the waves' instructions, one after another: 48 products of 32 cycles, 32 exponentials of 16 and some 300 others of 4 or more per wave
-// and 64 keys; two waves a SIMD (222 registers) hide little more of one another than this.  Five prompts of up to 2048 tokens, 32 q and 8 kv heads of
+// Bound: the waves' instructions, one after another: 48 products of 32 cycles, 32 exponentials of 16 and 275 others of 4 per wave and 64 keys
+// (counted) are 3150 cycles, of which a SIMD takes 2840: matrix instructions 54 % of its cycles, vector instructions 49 %, hardly at the same time,
+// though it has two waves (222 registers).  e4m3 46 % and 54 %.  Five prompts of up to 2048 tokens, 32 q and 8 kv heads of
 // 128: 173 us (e4m3 186), 0.65 PFLOP/s of the 1.35 of a large library product, 0.98 with the weights' second numbers counted.  Slower, measured with
 // weights of one number: products and exponentials of two tiles interleaved (137 -> 140), two groups of waves in turn (26.8 -> 28.4 for 256 tokens behind
 // 8000), workgroups that take several blocks (the registers spill: 138 -> 146).

@@ -2,8 +2,8 @@
 //
 // Both move every byte once and compute next to nothing: memory-bound, and in a decode step bound by the launch and two dependent
 // reads (where the row belongs, then its page).  A lane has 8 elements of a head's row (16 bytes of bf16), HD / 8 lanes a row.
-// Six prompts of the 8B model into e4m3, 110 MB: 23.3 us, 4.7 TB/s (a large copy 5.05); 16 sequences of it read back, 116 MB: 20.1 us, 5.8 TB/s; a row of
-// one sequence, or of 64: 5.2 us from Python, most of it the call.
+// Six prompts of the 8B model into e4m3, 110 MB: 23.3 us, 4.7 TB/s (a large copy 5.05); 16 sequences of it read back, 116 MB: 20.0 us, 5.8 TB/s; a row of
+// one sequence, or of 64: 6.0 us from Python, most of it the call (in a captured graph 2.4 and 4.0).
 #include "paged_common.h"
 
 constexpr int PAGED_TOKENS = 16;   // of a workgroup, at most
