@@ -34,6 +34,9 @@ struct PagedQuery {
 // and its ticket 1.0, the parts together 1.8, the rest start and end.
 typedef int i32x2_t __attribute__((ext_vector_type(2)));
 constexpr float PAGED_TAU2 = 8.0f;   // log2 of the largest weight before the reference point of the exponentials moves
+// Exponents are score * c2 - m * c2 with one rounding, m * c2 rounded once for all: a factor that all weights of a row share.  Where it could leave fp32
+// (it is 2 to the power of 2^-25 of m * c2) scores are taken less m first: from this |m * c2| on, at which a score of fp32 is itself off by more.
+constexpr float PAGED_FAR = 0x1p20f;
 constexpr int PAGED_OUT = (int)0x80000000;   // an offset outside every resource: comes as zeros
 constexpr int PAGED_COHERENT = 17;   // sc0 sc1: past this XCD's L2
 
@@ -449,7 +452,8 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
       top = rows_max(top);
       // (the reference point moves only when a tile's maximum exceeds it by more than tau: weights stay below 2^PAGED_TAU2)
       const bool grow = top > m + tau;   // m = -inf: any finite maximum
-      const float mn = grow ? top : m, nmc = mn == -INFINITY ? 0.0f : -mn * c2;
+      const float mn = grow ? top : m;
+      float nmc = mn == -INFINITY ? 0.0f : -mn * c2;
       if (__any(grow)) {
         const float corr = grow ? exp2_hw((m - mn) * c2) : 1.0f;   // m = -inf: 0
         l *= corr;
@@ -460,6 +464,12 @@ __global__ __launch_bounds__((DecodeTile<HD, E4M3>::NW * 64), (DecodeTile<HD, E4
           for (int d = 0; d < DT; ++d) o_low[d] *= corr;
       }
       m = mn;
+      const bool far = fabsf(nmc) >= PAGED_FAR;
+      if (__any(far)) {
+        nmc = far ? 0.0f : nmc;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sc[e >> 2][e & 3] = far ? sc[e >> 2][e & 3] - m : sc[e >> 2][e & 3];
+      }
       u32x4_t ph, pl;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -996,7 +1006,8 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
       top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
     }
     const bool grow = top > m + tau;   // m = -inf: any finite maximum
-    const float mn = grow ? top : m, nmc = mn == -INFINITY ? 0.0f : -mn * c2;
+    const float mn = grow ? top : m;
+    float nmc = mn == -INFINITY ? 0.0f : -mn * c2;
     if (__any(grow)) {
       const float corr = grow ? exp2_hw((m - mn) * c2) : 1.0f;   // m = -inf: 0
       l *= corr;
@@ -1006,6 +1017,14 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
         for (int v = 0; v < 16; ++v) o[d][v] *= corr;
     }
     m = mn;
+    const bool far = fabsf(nmc) >= PAGED_FAR;
+    if (__any(far)) {
+      nmc = far ? 0.0f : nmc;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sacc[n][v] = far ? sacc[n][v] - m : sacc[n][v];
+    }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       u32x4_t ph[2], pl[2];
@@ -1126,7 +1145,7 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
-        const float nmc = m == -INFINITY ? 0.0f : -m * c2;
+        const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll 1
         for (int key = t_first; key < t_end && key <= pmax; ++key) {
           const int page = my_key(key) ? page_of(key) : -1;
@@ -1144,7 +1163,7 @@ __global__ __launch_bounds__(256 * KSP, 2) void k_paged_prompt(const PagedCache 
               s = fmaf(bf_hi(q1), k4[3], s);
             }
           s += __shfl_xor(s, 32, LR_WAVE);
-          const float weight = exp2_hw(fmaf(s, c2, nmc));
+          const float weight = exp2_hw(fminf(s - ref, tau) * c2);   // (no larger than the products' ones, however this sum is rounded)
 #pragma unroll
           for (int d = 0; d < DT; ++d)
 #pragma unroll

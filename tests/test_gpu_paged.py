@@ -930,3 +930,34 @@ def test_rows_of_the_largest_and_smallest_numbers_are_written_as_defined(hip):
         assert torch.equal(cache.scales[page, 0, which, :4].cpu(), byte) and torch.equal(pages[page, 0, :4].cpu().float(), x.float())
         want = (x.double() * torch.exp2(byte.double() - 127)[:, None]).to(F32).to(BF)
         assert torch.equal(got.cpu(), want) and want[0].isinf().any() and want[3].isinf().any() and want[1:3].isfinite().all()
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("hd,lengths,new", [(64, [90, 33], None), (128, [2500], None), (64, [90, 33], [60, 33]), (128, [900], [9]), (128, [700], [700])])
+@pytest.mark.parametrize("scale,q_scale", [(2.0 ** 30, 1.0), (2.0 ** 40, 1.0), (2.0 ** 64, 1.0), (None, 2.0 ** 40)])
+def test_scores_beyond_what_exponents_tell_apart(hip, e4m3, hd, lengths, new, scale, q_scale):
+    """Scores of 2^30 and more: the value of a row's largest one, where that is clear of the next.  fp32 sums of hd products are off by hd * 2^-24 of
+    the sum of their sizes, at most; a gap of 2^-10 of it, times scale 2^20 and more, leaves the others no weight."""
+    hq = 2
+    case = Case(lengths, 1, hd, 16, e4m3, seed=65, new=new)
+    cache, batch = case.on(DEV, hq)
+    q = rnd(case.rows, hq * hd, seed=66, scale=q_scale)
+    y = cache.attend(batch, q.to(DEV), torch.empty(case.rows, hq * hd, dtype=BF, device=DEV), scale).cpu().view(-1, hq, hd)
+    assert y.isfinite().all()
+    k, v = (torch.nan_to_num(O.values(x, case.scales, i), nan=0.0)[:, 0] for i, x in enumerate((case.k, case.v)))
+    clear = 0
+    for b, n in enumerate(lengths):
+        ids = case.table[b, :-(-n // 16)].long()
+        ks, vs = k[ids].reshape(-1, hd)[:n], v[ids].reshape(-1, hd)[:n]
+        first, end = (b, b + 1) if new is None else case.starts[b:b + 2]
+        for r in range(first, end):
+            seen = n - (end - r) + 1
+            for h in range(hq):
+                x = q[r, h * hd:(h + 1) * hd].double()
+                s, size = ks[:seen] @ x, float((ks[:seen].abs() @ x.abs()).max())
+                top = s.argmax()
+                others = s[torch.arange(seen) != top]
+                if seen == 1 or s[top] - others.max() > size * 2.0 ** -10:
+                    assert torch.equal(y[r, h], vs[top].to(BF)), (r, h)
+                    clear += 1
+    assert clear >= case.rows * hq // 2
