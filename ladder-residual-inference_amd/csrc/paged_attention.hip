@@ -778,7 +778,7 @@ __device__ __forceinline__ bool prompt_block(const PagedCache& c, const PagedBat
     n = i < t.B ? t.starts[i + 1] - start : 0;
     n = start < 0 || start > rows || n < 0 ? 0 : n;
     const int length = i < t.B ? max(t.lengths[i], 0) : 0;   // (positions are the length's, also where the table has not all of its keys)
-    if (length > at.held && t.err) *t.err = LR_DEV_POS_RANGE;
+    if (n && length > at.held && t.err) *t.err = LR_DEV_POS_RANGE;
     ahead = length - n;
     n = min(n, rows - start);   // (a call may have fewer rows than starts says)
     blocks = (int)(((int64_t)n * G + PROMPT_ROWS - 1) / PROMPT_ROWS);

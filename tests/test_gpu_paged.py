@@ -961,3 +961,11 @@ def test_scores_beyond_what_exponents_tell_apart(hip, e4m3, hd, lengths, new, sc
                     assert torch.equal(y[r, h], vs[top].to(BF)), (r, h)
                     clear += 1
     assert clear >= case.rows * hq // 2
+
+
+def test_a_sequence_without_rows_has_no_position_out_of_range(hip):
+    """A sequence that takes no part may be longer than the table: nobody is told of it."""
+    case = Case([64, 33, 20], 2, 64, 16, False, seed=67, new=[0, 33, 0])
+    case.table, case.lengths = case.table[:, :4].contiguous(), [4000, 33, 65]
+    attend(case, 4)
+    hip.raise_on_device_error(DEV)
