@@ -132,6 +132,11 @@ class PagedKVCache(nn.Module):
         return (*self.k_pages.shape[1:], self.k_pages.dtype, self.k_pages.device)
 
     def desc(self):
+        """The pages' descriptor as they are now.  (They may be exchanged behind __setattr__, too: .data, set_(), a shallow copy's buffers.)"""
+        if self._desc is not None:
+            b, (k, v, s) = self._buffers, self._at
+            if b["k_pages"].data_ptr() != k or b["v_pages"].data_ptr() != v or s is not None and b["scales"].data_ptr() != s:
+                self._desc = None
         if self._desc is None:
             self._desc = _hip.paged_cache_desc(self.k_pages, self.v_pages, self.scales)
             self._shape = _PAGED_SHAPES.setdefault(self.shape, self.shape)     # (one tuple each: a call's check compares addresses)
@@ -155,17 +160,10 @@ class PagedKVCache(nn.Module):
         sequence); `rows`: how many rows a call has at most (given with starts).  Serves every cache of the same shape."""
         assert starts is None or rows is not None, "with starts, say how many rows a call has at most"
         assert starts is not None or rows in (None, table.shape[0]), "without starts there is one row per sequence"
-        self._desc = None     # (the pages as they are now)
         return PagedBatch(self, table, lengths, n_head, starts, table.shape[0] if rows is None else rows)
 
     def _check(self, batch: PagedBatch):
-        desc = self._desc
-        if desc is not None:     # (pages may be exchanged behind __setattr__, too: .data, set_(), a shallow copy's buffers)
-            b, (k, v, s) = self._buffers, self._at
-            if b["k_pages"].data_ptr() != k or b["v_pages"].data_ptr() != v or s is not None and b["scales"].data_ptr() != s:
-                desc = self._desc = None
-        if desc is None:
-            desc = self.desc()
+        desc = self.desc()
         if batch.shape is not self._shape:
             raise ValueError(f"a batch for pages {batch.shape}: got pages {self._shape}")
         return desc
