@@ -739,8 +739,8 @@ static int launch_paged_decode(const PagedCache& c, const PagedBatch& t, const P
 // Few rows: a workgroup's keys are cut among several, whose results a second launch puts together.
 //
 // Bound: the waves' instructions, one after another: 48 products of 32 cycles, 32 exponentials of 16 and 275 others of 4 per wave and 64 keys
-// (counted) are 3150 cycles, of which a SIMD takes 2860: matrix instructions 54 % of its cycles, vector instructions 49 %, hardly at the same time,
-// though it has two waves (222 registers).  e4m3 46 % and 54 %.  Five prompts of up to 2048 tokens, 32 q and 8 kv heads of
+// (counted) are 3150 cycles, of which a SIMD takes 2860: matrix instructions 54 % of its cycles, vector instructions 49 %, so that they run at the
+// same time hardly more than neither does, though it has two waves (222 registers).  e4m3 46 % and 54 %.  Five prompts of up to 2048 tokens, 32 q and 8 kv heads of
 // 128: 174 us (e4m3 186), 0.65 PFLOP/s of the 1.35 of a large library product, 0.98 with the weights' second numbers counted.  Slower, measured with
 // weights of one number: products and exponentials of two tiles interleaved (137 -> 140), two groups of waves in turn (26.8 -> 28.4 for 256 tokens behind
 // 8000), workgroups that take several blocks (the registers spill: 138 -> 146).

@@ -2,6 +2,7 @@
 
 What no sequence has in the pages is NaN, with the largest scale where rows have one; lengths lie around the edges of tiles and pages."""
 import math
+import random
 
 import pytest
 import torch
@@ -969,3 +970,117 @@ def test_a_sequence_without_rows_has_no_position_out_of_range(hip):
     case.table, case.lengths = case.table[:, :4].contiguous(), [4000, 33, 65]
     attend(case, 4)
     hip.raise_on_device_error(DEV)
+
+
+# ------------------------------------------------------------------------------------------------ calls that are allowed
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_captured_prompts_follow_what_the_device_holds(hip, e4m3):
+    """write, attend and read of a call with starts, captured once: lengths, starts and the table change between replays, the program's own
+    eager calls run between them."""
+    hq, hkv, hd, page, rows, B = 8, 2, 64, 16, 90, 5
+    from gpt_fast.utils import PagedKVCache
+    dtype = E4M3 if e4m3 else BF
+    caches = [PagedKVCache(400, page, hkv, hd, dtype, device=DEV) for _ in range(2)]
+    g = torch.Generator().manual_seed(70)
+    i32 = lambda x: torch.as_tensor(x, dtype=torch.int32).to(DEV)
+    table, lengths, starts = i32(torch.zeros(B, 80)), i32(torch.ones(B)), i32(torch.arange(B + 1))
+    batch = caches[0].batch(table, lengths, hq, starts=starts, rows=rows)
+    qkv = torch.zeros(rows, (hq + 2 * hkv) * hd, dtype=BF, device=DEV)
+    angle = torch.rand(1300, hd // 2, generator=g) * 6.28
+    rope = torch.stack([angle.cos(), angle.sin()], -1).to(DEV)
+    outs = [[torch.zeros(rows, w, dtype=BF, device=DEV) for w in (hq * hd, hq * hd, hkv * hd, hkv * hd)] for _ in range(2)]
+
+    def once(cache, b, q, y, k, v):
+        cache.write(b, qkv, q, rope)
+        cache.attend(b, q, y)
+        cache.read(b, k, v)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        once(caches[0], batch, *outs[0])
+    r = random.Random(71)
+    for _ in range(8):
+        new = [r.choice([0, 1, r.randint(0, 17)]) for _ in range(B)]
+        ahead = [r.choice([0, r.randint(0, 40), r.randint(0, 1180)]) for _ in range(B)]
+        at = [sum(new[:b]) for b in range(B + 1)]
+        table.copy_(torch.randperm(400, generator=g)[:B * 80].view(B, 80).to(torch.int32))
+        lengths.copy_(i32([a + n for a, n in zip(ahead, new)]))
+        starts.copy_(i32(at))
+        qkv.copy_(torch.randn(qkv.shape, generator=g))
+        for a, b in zip(caches[0].buffers(), caches[1].buffers()):
+            b.copy_(a)
+        for out in outs:
+            for t in out:
+                t.fill_(3)
+        once(caches[1], caches[1].batch(table.clone(), lengths.clone(), hq, starts=starts.clone(), rows=rows), *outs[1])
+        graph.replay()
+        for a, b in zip((*caches[0].buffers(), *outs[0]), (*caches[1].buffers(), *outs[1])):
+            assert torch.equal(bits(a), bits(b))
+        assert all((t[at[-1]:] == 3).all() and t[:at[-1]].isfinite().all() for t in outs[0])
+
+
+@pytest.mark.parametrize("new", [None, [1, 40]])
+def test_rows_side_by_side_in_one_matrix(hip, new):
+    """q and y as columns of the same matrix, and k and v that are read back: what lies between stays."""
+    hq, hkv, hd = 4, 2, 64
+    case = Case([30, 77], hkv, hd, 16, False, seed=72, new=new)
+    cache, batch = case.on(DEV, hq)
+    width = hq * hd
+    m = torch.full((case.rows, 2 * width + 2 * hkv * hd + 24), 3.0, dtype=BF, device=DEV)
+    m[:, 8:8 + width] = rnd(case.rows, width, seed=73).to(DEV)
+    want = cache.attend(batch, m[:, 8:8 + width].contiguous(), torch.empty(case.rows, width, dtype=BF, device=DEV)).clone()
+    k0, v0 = (torch.empty(case.rows, hkv * hd, dtype=BF, device=DEV) for _ in range(2))
+    cache.read(batch, k0, v0)
+    before = m.clone()
+    cache.attend(batch, m[:, 8:8 + width], m[:, 16 + width:16 + 2 * width])
+    cache.read(batch, m[:, 16 + 2 * width:16 + 2 * width + hkv * hd], m[:, 24 + 2 * width + hkv * hd:])
+    before[:, 16 + width:16 + 2 * width] = want
+    before[:, 16 + 2 * width:16 + 2 * width + hkv * hd], before[:, 24 + 2 * width + hkv * hd:] = k0, v0
+    assert torch.equal(bits(m), bits(before))
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("single", [True, False])
+def test_as_many_sequences_as_a_call_has(hip, e4m3, single):
+    """65535 sequences of one or two tokens, every ninth of none."""
+    from gpt_fast.utils import PagedKVCache
+    B, hq, hd, page = 65535, 2, 64, 16
+    cache = PagedKVCache(B, page, 1, hd, E4M3 if e4m3 else BF, device=DEV)
+    g = torch.Generator().manual_seed(74)
+    i32 = lambda x: torch.as_tensor(x, dtype=torch.int32).to(DEV)
+    table = torch.randperm(B, generator=g).to(torch.int32)[:, None]
+    lengths = torch.randint(1, 3, (B,), generator=g)
+    lengths[::9] = 0
+    ends = torch.cat([torch.zeros(1, dtype=torch.int64), lengths.cumsum(0)])
+    rows = int(ends[-1])
+    whole = cache.batch(i32(table), i32(lengths), hq, starts=i32(ends), rows=rows)
+    qkv = torch.randn(rows, (hq + 2) * hd, generator=g).to(BF).to(DEV)
+    q = torch.empty(rows, hq * hd, dtype=BF, device=DEV)
+    cache.write(whole, qkv, q)
+    k, v = (torch.empty(rows, hd, dtype=BF, device=DEV) for _ in range(2))
+    cache.read(whole, k, v)
+    if not e4m3:
+        assert torch.equal(k, qkv[:, hq * hd:(hq + 1) * hd]) and torch.equal(v, qkv[:, (hq + 1) * hd:])
+    last = ends[1:][lengths > 0].to(DEV) - 1
+    if single:
+        x = torch.zeros(B, hq * hd, dtype=BF, device=DEV)
+        there = (lengths > 0).to(DEV)
+        x[there] = q[last]
+        y = cache.attend(cache.batch(i32(table), i32(lengths), hq), x, torch.full_like(x, 3))
+        assert (y[~there] == 0).all()
+        y = y[there]
+    else:
+        y = cache.attend(whole, q, torch.full_like(q, 3))
+        first = ends[:-1][lengths > 0].to(DEV)
+        assert torch.equal(y[first], v[first].repeat(1, hq))        # a first token sees itself alone
+        y = y[last]
+    # a second token: two keys
+    two = (lengths[lengths > 0] == 2).to(DEV)
+    assert torch.equal(y[~two], v[last][~two].repeat(1, hq))
+    qf, kf, vf = q[last][two].double().view(-1, hq, hd), k.double(), v.double()
+    k1, k0, v1, v0 = kf[last][two], kf[last - 1][two], vf[last][two], vf[last - 1][two]
+    d = ((qf * (k1 - k0)[:, None]).sum(-1, keepdim=True) * hd ** -0.5).sigmoid()
+    want, spread = d * v1[:, None] + (1 - d) * v0[:, None], d * v1[:, None].abs() + (1 - d) * v0[:, None].abs()
+    size = float(torch.maximum((qf.abs() * k1.abs()[:, None]).sum(-1), (qf.abs() * k0.abs()[:, None]).sum(-1)).max()) * hd ** -0.5
+    assert ((y[two].double().view(want.shape) - want).abs() <= bound(want, spread, size, 2, hd, WEIGHT)).all()
